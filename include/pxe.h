@@ -6,7 +6,8 @@
  * site(s) it stands in for, by path inside the trieck/pixienn tree.
  *
  * Conventions
- *  - All tensors are fp32, NCHW.  A "batch stride" is the distance in ELEMENTS
+ *  - All tensors are fp32, NCHW (the row operators at the end of this file say otherwise: rows of
+ *    contiguous values of a pxe_dtype).  A "batch stride" is the distance in ELEMENTS
  *    between consecutive images of a tensor; 0 means "densely packed"
  *    (channels*height*width).  A non-dense stride lets a kernel read from or
  *    write into a channel slot of a wider concat buffer, which is how route
@@ -615,6 +616,154 @@ PXE_API int pxe_batchnorm_forward_training(pxe_stream_t stream, const pxe_bn_tra
 /* Three launches: per-channel sums of dy and dy * (x - mean), per-channel constants (and the parameter gradients),
  * dx = k1 * dy + k2 * x + k3. */
 PXE_API int pxe_batchnorm_backward(pxe_stream_t stream, const pxe_bn_backward_desc* desc);
+
+/* ------------------------------------------------------------------------------------------
+ * Row operators in 32- and 16-bit types: the tail of a training step around a classifier, and its answers when served.
+ * Not in the reference; they stand beside batch norm with its shortcut (pxe_batchnorm_*, pxe_shortcut), the softmax
+ * layer and its loss (pxe_softmax, pxe_softmax_decode, pxe_softmax_cross_entropy) and the Adam step
+ * (pxe_adam_update).  A tensor is `rows` rows of contiguous values of one pxe_dtype; a "row stride" is the distance in
+ * ELEMENTS between consecutive rows, 0 = densely packed.  Channels-last pixels are such rows.  Sums, statistics and
+ * moments are held in fp32, and every sum is taken in a fixed order.  Tensors need the alignment of their element
+ * type only; rows on 16-byte boundaries are faster.  A destination may be a source itself (same pointer and strides)
+ * where its comment says so; any other overlap of a destination is refused.
+ * ------------------------------------------------------------------------------------------ */
+enum pxe_dtype { PXE_F32 = 0, PXE_BF16 = 1, PXE_F16 = 2 };
+
+/* Root-mean-square norm over the channels of every row, with the addition in front of it:
+ *   h = x + residual (rounded to `type`; x itself without a residual), rstd = 1 / sqrt(mean(h^2) + eps),
+ *   y = h * rstd * weight.
+ * y goes to `y` in `type`, or to `q` as 8-bit floating point (e4m3: 4 exponent, 3 mantissa bits, largest value 448)
+ * with one scale for every `group` channels (the last group of a row may be short; 0 = one for the row):
+ *   scale = max(max |y| / 448, 2^-126), q = e4m3(y / scale).
+ * A row that holds a NaN or whose sum of squares is not finite gives NaN where IEEE arithmetic does; nothing else does.
+ * h and y may be x or residual; q may not be a source.  rows == 0: nothing to do.  channels <= 262144. */
+typedef struct pxe_rms_norm_desc {
+    const void* x;
+    const void* residual;      /* or NULL */
+    const void* weight;        /* [channels], or NULL for ones */
+    void* h;                   /* destination of the sum (needed with a residual, NULL without) */
+    void* y;                   /* destination in `type`, or NULL when q is given */
+    void* q;                   /* destination in e4m3 bytes, or NULL when y is given */
+    float* scale;              /* with q: [rows, ceil(channels / group)] dense */
+    float* rstd;               /* [rows] out, or NULL */
+    long long x_row_stride, residual_row_stride, h_row_stride, y_row_stride, q_row_stride;
+    long long rows;
+    int channels;
+    int type;                  /* enum pxe_dtype of x, residual, h, y */
+    int weight_type;           /* enum pxe_dtype of weight: PXE_F32 or `type` */
+    int group;                 /* 0, 32, 64 or 128 */
+    float eps;
+} pxe_rms_norm_desc;
+PXE_API int pxe_rms_norm(pxe_stream_t stream, const pxe_rms_norm_desc* desc);
+
+/* Its gradient: with u = dy * weight,
+ *   dx = rstd * (u - h * rstd^2 * mean(u * h)) + dresidual,   dweight[c] = sum over rows of dy * h * rstd.
+ * dx is the gradient of x and of the residual alike; dresidual is what reaches h past the norm.  dweight is assigned,
+ * or added to with accumulate != 0 (as pxe_batchnorm_backward does); rows == 0 leaves zeros, or what was there.
+ * dx may be dy, h or dresidual. */
+typedef struct pxe_rms_norm_backward_desc {
+    const void* dy;
+    const void* h;             /* the h that the forward call wrote (x without a residual) */
+    const void* dresidual;     /* or NULL */
+    const void* weight;        /* or NULL for ones */
+    const float* rstd;         /* [rows] from the forward call */
+    void* dx;
+    float* dweight;            /* [channels], or NULL */
+    long long dy_row_stride, h_row_stride, dresidual_row_stride, dx_row_stride;
+    long long rows;
+    int channels;
+    int type, weight_type;
+    int accumulate;
+    void* workspace;           /* pxe_rms_norm_backward_workspace_bytes(rows, channels), 16-byte aligned; unused (may be */
+    size_t workspace_bytes;    /* NULL) without dweight.  Calls that may run at the same time need one each */
+} pxe_rms_norm_backward_desc;
+PXE_API size_t pxe_rms_norm_backward_workspace_bytes(long long rows, int channels);
+PXE_API int pxe_rms_norm_backward(pxe_stream_t stream, const pxe_rms_norm_backward_desc* desc);
+
+/* Log probabilities of given classes, entropy and the most likely alternatives.  With d_j = (x_j - max x) / temperature
+ * and S = sum exp(d_j) over the row's classes:
+ *   logp = d_target - log S,  entropy = log S - sum(exp(d_j) * d_j) / S,
+ *   top_index / top_logp: the `top` largest values, largest first, ties to the lower class.
+ * Row r lies at x + (r / inner) * outer_stride + (r % inner) * row_stride, so that a slice of a [batch, length, classes]
+ * tensor needs no copy.  A row with target < 0 is not used: it is not read, its logp, entropy and top_logp are 0, its
+ * top_index -1.  A target >= classes gives a logp of NaN (nothing is read there).  Values of -inf have probability 0; a row
+ * of nothing else has logp -inf and entropy 0.  A row with a NaN or +inf has logp and entropy NaN; a NaN counts as
+ * larger than every number among the alternatives.  rows == 0: nothing to do. */
+typedef struct pxe_log_probs_desc {
+    const void* x;
+    const void* target;        /* [rows] int32 or int64, or NULL: every row is used, no logp */
+    float* logp;               /* [rows]; NULL without target */
+    float* entropy;            /* [rows] or NULL */
+    float* stats;              /* [rows, 3] or NULL: max x, log2 S, entropy, for pxe_log_probs_backward */
+    float* top_logp;           /* [rows, top] or NULL when top == 0 */
+    int* top_index;            /* [rows, top] or NULL when top == 0 */
+    long long rows, inner, outer_stride, row_stride;   /* inner == 0: one group of rows */
+    int classes;
+    int type;                  /* enum pxe_dtype of x */
+    int target_is_int64;
+    int top;                   /* 0..32, at most classes */
+    float temperature;         /* > 0 */
+} pxe_log_probs_desc;
+PXE_API int pxe_log_probs(pxe_stream_t stream, const pxe_log_probs_desc* desc);
+
+/* Its gradient with respect to x, from dlogp and dentropy (either may be NULL, and a NULL target has no dlogp):
+ *   dx_j = (dlogp * ([j == target] - p_j) - dentropy * p_j * (log p_j + entropy)) / temperature.
+ * Rows that are not used, and rows of -inf throughout, have a gradient of 0; a target >= classes gives NaN.
+ * dx: `type`, addressed like x with its own strides; dx may be x. */
+typedef struct pxe_log_probs_backward_desc {
+    const void* x;
+    const void* target;
+    const float* stats;        /* from the forward call */
+    const float* dlogp;        /* [rows] or NULL */
+    const float* dentropy;     /* [rows] or NULL */
+    void* dx;
+    long long rows, inner, outer_stride, row_stride, dx_outer_stride, dx_row_stride;
+    int classes;
+    int type;
+    int target_is_int64;
+    float temperature;
+} pxe_log_probs_backward_desc;
+PXE_API int pxe_log_probs_backward(pxe_stream_t stream, const pxe_log_probs_backward_desc* desc);
+
+/* An AdamW step over many tensors.  For every element, with g = grad_scale * grad and p the master copy where there is
+ * one, the parameter otherwise:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p - rate * ((m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay * p),
+ * and the parameter receives p rounded to its type.  (pxe_adam_update adds its step, as the reference's deltas are the
+ * negative gradient: grad_scale = -1 serves such deltas.)
+ * State in 32 bits: m and v are fp32.  In 8 bits: m and sqrt(v) are e4m3 bytes, each times the scale of its block of
+ * PXE_ADAMW_BLOCK elements (scale = max(largest / 448, 2^-126) of the new values; a v above zero keeps a code above
+ * zero); arithmetic stays in fp32.  A gradient that is not finite spoils its element, and in 8 bits its block.
+ * `tensors` is a HOST array that the call reads before it returns; entries with n == 0 are passed over.  Nothing may
+ * overlap anything else: parameters, states and masters that do are refused.  The step is one launch for every
+ * PXE_ADAMW_TENSORS_PER_LAUNCH tensors, with no workspace. */
+#define PXE_ADAMW_BLOCK 256
+#define PXE_ADAMW_TENSORS_PER_LAUNCH 400
+typedef struct pxe_adamw_tensor {
+    void* param;
+    const void* grad;
+    void* m;
+    void* v;
+    float* m_scale;            /* 8-bit state: [ceil(n / PXE_ADAMW_BLOCK)] each; NULL for 32-bit state */
+    float* v_scale;
+    float* master;             /* fp32 copy of a 16-bit parameter, in all entries or in none */
+    long long n;
+} pxe_adamw_tensor;
+typedef struct pxe_adamw_desc {
+    const pxe_adamw_tensor* tensors;
+    int count;
+    int param_type, grad_type; /* enum pxe_dtype */
+    int state_bits;            /* 32 or 8 */
+    float rate, beta1, beta2, eps, weight_decay, grad_scale;
+    long long t;               /* counts steps from 1 */
+    /* device scalars that replace the values above when they are not NULL (a step captured in a CUDA graph reads the
+     * current ones at every replay), and a flag that, not 0, leaves everything as it is */
+    const float* rate_device;
+    const long long* t_device;
+    const float* grad_scale_device;
+    const float* skip_device;
+} pxe_adamw_desc;
+PXE_API int pxe_adamw_update(pxe_stream_t stream, const pxe_adamw_desc* desc);
 
 #ifdef __cplusplus
 }

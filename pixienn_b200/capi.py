@@ -125,6 +125,58 @@ class BnBackwardDesc(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+F32, BF16, F16 = 0, 1, 2                  # enum pxe_dtype
+
+
+class RmsNormDesc(C.Structure):
+    """pxe_rms_norm_desc of include/pxe.h."""
+    _fields_ = [("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("h", C.c_void_p), ("y", C.c_void_p),
+                ("q", C.c_void_p), ("scale", C.c_void_p), ("rstd", C.c_void_p),
+                ("x_row_stride", C.c_longlong), ("residual_row_stride", C.c_longlong), ("h_row_stride", C.c_longlong),
+                ("y_row_stride", C.c_longlong), ("q_row_stride", C.c_longlong), ("rows", C.c_longlong),
+                ("channels", C.c_int), ("type", C.c_int), ("weight_type", C.c_int), ("group", C.c_int), ("eps", C.c_float)]
+
+
+class RmsNormBackwardDesc(C.Structure):
+    """pxe_rms_norm_backward_desc of include/pxe.h."""
+    _fields_ = [("dy", C.c_void_p), ("h", C.c_void_p), ("dresidual", C.c_void_p), ("weight", C.c_void_p), ("rstd", C.c_void_p),
+                ("dx", C.c_void_p), ("dweight", C.c_void_p),
+                ("dy_row_stride", C.c_longlong), ("h_row_stride", C.c_longlong), ("dresidual_row_stride", C.c_longlong),
+                ("dx_row_stride", C.c_longlong), ("rows", C.c_longlong), ("channels", C.c_int), ("type", C.c_int),
+                ("weight_type", C.c_int), ("accumulate", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class LogProbsDesc(C.Structure):
+    """pxe_log_probs_desc of include/pxe.h."""
+    _fields_ = [("x", C.c_void_p), ("target", C.c_void_p), ("logp", C.c_void_p), ("entropy", C.c_void_p), ("stats", C.c_void_p),
+                ("top_logp", C.c_void_p), ("top_index", C.c_void_p), ("rows", C.c_longlong), ("inner", C.c_longlong),
+                ("outer_stride", C.c_longlong), ("row_stride", C.c_longlong), ("classes", C.c_int), ("type", C.c_int),
+                ("target_is_int64", C.c_int), ("top", C.c_int), ("temperature", C.c_float)]
+
+
+class LogProbsBackwardDesc(C.Structure):
+    """pxe_log_probs_backward_desc of include/pxe.h."""
+    _fields_ = [("x", C.c_void_p), ("target", C.c_void_p), ("stats", C.c_void_p), ("dlogp", C.c_void_p), ("dentropy", C.c_void_p),
+                ("dx", C.c_void_p), ("rows", C.c_longlong), ("inner", C.c_longlong), ("outer_stride", C.c_longlong),
+                ("row_stride", C.c_longlong), ("dx_outer_stride", C.c_longlong), ("dx_row_stride", C.c_longlong),
+                ("classes", C.c_int), ("type", C.c_int), ("target_is_int64", C.c_int), ("temperature", C.c_float)]
+
+
+class AdamwTensor(C.Structure):
+    """pxe_adamw_tensor of include/pxe.h."""
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("master", C.c_void_p), ("n", C.c_longlong)]
+
+
+class AdamwDesc(C.Structure):
+    """pxe_adamw_desc of include/pxe.h."""
+    _fields_ = [("tensors", C.c_void_p), ("count", C.c_int), ("param_type", C.c_int), ("grad_type", C.c_int), ("state_bits", C.c_int),
+                ("rate", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float), ("weight_decay", C.c_float),
+                ("grad_scale", C.c_float), ("t", C.c_longlong), ("rate_device", C.c_void_p), ("t_device", C.c_void_p),
+                ("grad_scale_device", C.c_void_p), ("skip_device", C.c_void_p)]
+
+
+ADAMW_BLOCK = 256                         # PXE_ADAMW_BLOCK
 PLAN_MAX_SOURCES, PLAN_MAX_DESTS, PLAN_MAX_SPP = 16, 8, 4
 
 
@@ -210,6 +262,12 @@ PROTOTYPES = {
     "pxe_batchnorm_workspace_bytes": (C.c_size_t, [_i] * 4),
     "pxe_batchnorm_forward_training": (_i, [_vp, C.POINTER(BnTrainDesc)]),
     "pxe_batchnorm_backward": (_i, [_vp, C.POINTER(BnBackwardDesc)]),
+    "pxe_rms_norm": (_i, [_vp, C.POINTER(RmsNormDesc)]),
+    "pxe_rms_norm_backward_workspace_bytes": (_sz, [_ll, _i]),
+    "pxe_rms_norm_backward": (_i, [_vp, C.POINTER(RmsNormBackwardDesc)]),
+    "pxe_log_probs": (_i, [_vp, C.POINTER(LogProbsDesc)]),
+    "pxe_log_probs_backward": (_i, [_vp, C.POINTER(LogProbsBackwardDesc)]),
+    "pxe_adamw_update": (_i, [_vp, C.POINTER(AdamwDesc)]),
 }
 
 # the planner of include/pxe_plan.h (host code)

@@ -1,0 +1,333 @@
+// An AdamW step over many tensors in one launch, with states in 32 or 8 bits.
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p -= rate ((m / c1) / (sqrt(v / c2) + eps) + decay p)
+//
+// Bound by memory: every element's parameter, gradient and moments are read once and all but the gradient written once
+// (28 bytes in fp32, 16 with states in 8 bits).  The tensors' addresses travel as the kernel's parameters (72 bytes
+// each, 400 to a launch), so a call needs no table in device memory, no copy and no workspace, and a captured call keeps
+// its own.  A block of 256 threads takes chunks of 4096 elements; it finds a chunk's tensor by bisection over the first
+// chunk of each.  A warp takes 256 elements at a time, eight to a lane: that is also the block of elements that shares a
+// scale in 8 bits, so the new scale is one reduction over the warp and nothing is read twice.
+//
+// In 8 bits m is held as an e4m3 code times its block's scale, and v as the code of its root: the update needs the root,
+// and its codes then reach 2^-18 of the block's largest value (2^-36 in v).  A v above zero keeps the smallest code
+// instead of rounding to zero, which would leave a later step to divide by eps alone.
+#include <algorithm>
+#include <exception>
+#include <vector>
+
+#include "pxe_types.cuh"
+
+namespace pxe {
+namespace {
+
+constexpr int kUnit = PXE_ADAMW_BLOCK;                     // elements a warp takes at a time
+constexpr int kThreads = 256;
+constexpr int kChunk = 4096;
+
+struct Entry {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* ms;
+    float* vs;
+    float* w;
+    long long n;
+    int first_chunk;
+    int vector;                                            // every pointer allows whole accesses
+};
+
+template <int MAX>
+struct AdamwParams {
+    float rate, b1, b2, omb1, omb2, eps, decay, grad_scale, inv_c1, inv_c2, log_b1, log_b2;
+    const float* rate_device;
+    const long long* t_device;
+    const float* grad_scale_device;
+    const float* skip_device;
+    int count, chunks;
+    Entry e[MAX];
+};
+
+struct Step {
+    float rate, b1, b2, omb1, omb2, eps, decay, grad_scale, inv_c1, inv_c2;
+    // the new moments and parameter of one element
+    __device__ __forceinline__ void operator()(float& p, float g, float& m, float& v) const
+    {
+        g *= grad_scale;
+        m = fmaf(omb1, g, b1 * m);
+        v = fmaf(omb2 * g, g, b2 * v);
+        p -= rate * (m * inv_c1 / (sqrtf(v * inv_c2) + eps) + decay * p);
+    }
+};
+
+__device__ __forceinline__ float warp_max(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// N elements of one access of a type
+template <typename T, int N>
+__device__ __forceinline__ void load(const void* base, long long i, float (&f)[N])
+{
+    constexpr int PER = N * sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int k = 0; k < N / PER; ++k) {
+        float part[PER];
+        unpack<T, PER>(gldv<Raw<T, PER>>(static_cast<const T*>(base) + i + k * PER), part);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) f[k * PER + j] = part[j];
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store(void* base, long long i, const float (&f)[N])
+{
+    constexpr int PER = N * sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int k = 0; k < N / PER; ++k) {
+        float part[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) part[j] = f[k * PER + j];
+        gstv(static_cast<T*>(base) + i + k * PER, pack<T, PER>(part));
+    }
+}
+
+// One unit of 256 elements from `first`: COUNT accesses of N elements to a lane, `stride` elements apart.  MASK: the
+// unit reaches past the tensor's end.
+template <typename P, typename G, bool SMALL, bool MASTER, int N, bool MASK>
+__device__ __forceinline__ void unit(const Entry& e, long long first, int lane, const Step& step)
+{
+    constexpr int COUNT = 8 / N, STRIDE = 32 * N;
+    float p[COUNT][N], g[COUNT][N], m[COUNT][N], v[COUNT][N];
+    float ms = 0.0f, vs = 0.0f;
+    const long long block = first / kUnit;
+    if constexpr (SMALL) { ms = gld(e.ms + block); vs = gld(e.vs + block); }
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) {
+        const long long i = first + k * STRIDE + lane * N;
+        if (MASK && i >= e.n) {                            // N == 1 there
+#pragma unroll
+            for (int j = 0; j < N; ++j) p[k][j] = g[k][j] = m[k][j] = v[k][j] = 0.0f;
+            continue;
+        }
+        if constexpr (MASTER) load<float, N>(e.w, i, p[k]);
+        else load<P, N>(e.p, i, p[k]);
+        load<G, N>(e.g, i, g[k]);
+        if constexpr (SMALL) {
+            unpack_e4m3<N>(gldv<typename RawOf<N>::type>(static_cast<const uint8_t*>(e.m) + i), m[k]);
+            unpack_e4m3<N>(gldv<typename RawOf<N>::type>(static_cast<const uint8_t*>(e.v) + i), v[k]);
+#pragma unroll
+            for (int j = 0; j < N; ++j) { m[k][j] *= ms; v[k][j] *= vs; v[k][j] *= v[k][j]; }
+        } else {
+            load<float, N>(e.m, i, m[k]);
+            load<float, N>(e.v, i, v[k]);
+        }
+    }
+    float m_max = 0.0f, v_max = 0.0f;
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) {
+        const long long i = first + k * STRIDE + lane * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) step(p[k][j], g[k][j], m[k][j], v[k][j]);
+        if (MASK && i >= e.n) continue;
+        if constexpr (MASTER) store<float, N>(e.w, i, p[k]);
+        store<P, N>(e.p, i, p[k]);
+        if constexpr (SMALL) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                v[k][j] = sqrtf(v[k][j]);
+                m_max = max_nan(m_max, fabsf(m[k][j]));
+                v_max = max_nan(v_max, v[k][j]);
+            }
+        } else {
+            store<float, N>(e.m, i, m[k]);
+            store<float, N>(e.v, i, v[k]);
+        }
+    }
+    if constexpr (SMALL) {
+        ms = max_nan(warp_max(m_max) / kE4m3Max, kScaleMin);
+        vs = max_nan(warp_max(v_max) / kE4m3Max, kScaleMin);
+        const float mi = 1.0f / ms, vi = 1.0f / vs;
+        constexpr float kSmallest = 0.001953125f;          // 2^-9
+        if (lane == 0) { gst(e.ms + block, ms); gst(e.vs + block, vs); }
+#pragma unroll
+        for (int k = 0; k < COUNT; ++k) {
+            const long long i = first + k * STRIDE + lane * N;
+            if (MASK && i >= e.n) continue;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                m[k][j] *= mi;
+                v[k][j] = v[k][j] > 0.0f ? max_nan(v[k][j] * vi, kSmallest) : v[k][j];
+            }
+            gstv(static_cast<uint8_t*>(e.m) + i, pack_e4m3<N>(m[k]));
+            gstv(static_cast<uint8_t*>(e.v) + i, pack_e4m3<N>(v[k]));
+        }
+    }
+}
+
+template <typename P, typename G, bool SMALL, bool MASTER, int MAX>
+__global__ void __launch_bounds__(kThreads)
+adamw_kernel(const __grid_constant__ AdamwParams<MAX> a)
+{
+    if (a.skip_device && gld(a.skip_device) != 0.0f) return;
+    // chosen as values: a member of Step overwritten under a condition kept the parameter's value (nvcc 12.9)
+    const float rate = a.rate_device ? gld(a.rate_device) : a.rate;
+    const float grad_scale = a.grad_scale_device ? gld(a.grad_scale_device) : a.grad_scale;
+    float inv_c1 = a.inv_c1, inv_c2 = a.inv_c2;
+    if (a.t_device) {                                      // 1 - b^t without the cancellation of the difference
+        const float t = (float)gld(a.t_device);
+        inv_c1 = -1.0f / expm1f(t * a.log_b1);
+        inv_c2 = -1.0f / expm1f(t * a.log_b2);
+    }
+    const Step step{rate, a.b1, a.b2, a.omb1, a.omb2, a.eps, a.decay, grad_scale, inv_c1, inv_c2};
+    constexpr int N = sizeof(P) == 4 ? 4 : 8;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+        int lo = 0, hi = a.count;                          // the last entry that begins at or before this chunk
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.e[mid].first_chunk <= chunk) lo = mid; else hi = mid;
+        }
+        const Entry& e = a.e[lo];
+        const long long begin = (long long)(chunk - e.first_chunk) * kChunk;
+        const long long end = begin + kChunk < e.n ? begin + kChunk : e.n;
+        for (long long first = begin + warp * kUnit; first < end; first += kThreads / 32 * kUnit) {
+            if (first + kUnit > e.n) unit<P, G, SMALL, MASTER, 1, true>(e, first, lane, step);
+            else if (e.vector) unit<P, G, SMALL, MASTER, N, false>(e, first, lane, step);
+            else unit<P, G, SMALL, MASTER, 1, false>(e, first, lane, step);
+        }
+    }
+}
+
+template <typename P, typename G, bool SMALL, bool MASTER>
+int launch(cudaStream_t s, AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>& a, const DeviceInfo& di)
+{
+    const unsigned grid = (unsigned)std::min<long long>(a.chunks, (long long)di.sm_count * 8);
+    adamw_kernel<P, G, SMALL, MASTER, PXE_ADAMW_TENSORS_PER_LAUNCH><<<grid, kThreads, 0, s>>>(a);
+    PXE_LAUNCH_OK("adamw_kernel");
+    return PXE_OK;
+}
+
+template <typename P, typename G>
+int launch(cudaStream_t s, AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>& a, const DeviceInfo& di, bool small, bool master)
+{
+    if constexpr (sizeof(P) == 4) {
+        return small ? launch<P, G, true, false>(s, a, di) : launch<P, G, false, false>(s, a, di);
+    } else {
+        if (master) return small ? launch<P, G, true, true>(s, a, di) : launch<P, G, false, true>(s, a, di);
+        return small ? launch<P, G, true, false>(s, a, di) : launch<P, G, false, false>(s, a, di);
+    }
+}
+
+struct Range {
+    uintptr_t lo, hi;
+    bool written;
+};
+
+// True when a written range shares a byte with any other.
+bool ranges_conflict(std::vector<Range>& r)
+{
+    bool ordered = true;
+    for (size_t i = 1; i < r.size() && ordered; ++i) ordered = r[i - 1].hi <= r[i].lo;
+    if (ordered) return false;
+    std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
+    uintptr_t any = 0, written = 0;                        // the furthest ends so far
+    for (const Range& x : r) {
+        if (x.lo < written || (x.written && x.lo < any)) return true;
+        any = std::max(any, x.hi);
+        if (x.written) written = std::max(written, x.hi);
+    }
+    return false;
+}
+
+}  // namespace
+}  // namespace pxe
+
+using namespace pxe;
+
+extern "C" int pxe_adamw_update(pxe_stream_t stream, const pxe_adamw_desc* dp)
+{
+    PXE_REQUIRE(dp != nullptr, "adamw_update: null descriptor");
+    const pxe_adamw_desc& d = *dp;
+    PXE_REQUIRE(d.count >= 0 && (d.count == 0 || d.tensors), "adamw_update: null or negative list of tensors");
+    PXE_REQUIRE(valid_dtype(d.param_type) && valid_dtype(d.grad_type), "adamw_update: unknown type");
+    if (d.param_type != PXE_F32 && d.grad_type != d.param_type && d.grad_type != PXE_F32)
+        return set_error(PXE_ERR_UNSUPPORTED, "adamw_update: gradients of one 16-bit type for parameters of the other");
+    PXE_REQUIRE(d.state_bits == 32 || d.state_bits == 8, "adamw_update: state_bits %d is neither 32 nor 8", d.state_bits);
+    PXE_REQUIRE(d.beta1 >= 0.0f && d.beta1 < 1.0f && d.beta2 >= 0.0f && d.beta2 < 1.0f, "adamw_update: beta1 and beta2 lie in [0, 1)");
+    PXE_REQUIRE(d.eps >= 0.0f, "adamw_update: eps is negative or NaN");
+    PXE_REQUIRE(d.t_device || d.t >= 1, "adamw_update: step %lld (the first step is 1)", d.t);
+    const bool small = d.state_bits == 8;
+    const int psize = dtype_bytes(d.param_type), gsize = dtype_bytes(d.grad_type), ssize = small ? 1 : 4;
+    bool master = false, first = true;
+    try {
+        std::vector<Range> ranges;
+        for (int family = 0; family < 7; ++family) {       // a family at a time: flat buffers come out in order
+            for (int i = 0; i < d.count; ++i) {
+                const pxe_adamw_tensor& t = d.tensors[i];
+                PXE_REQUIRE(t.n >= 0, "adamw_update: tensor %d has %lld elements", i, t.n);
+                if (t.n == 0) continue;
+                const long long blocks = (t.n + kUnit - 1) / kUnit;
+                if (family == 0) {
+                    PXE_REQUIRE(t.param && t.grad && t.m && t.v, "adamw_update: tensor %d has a null pointer", i);
+                    PXE_REQUIRE(small == (t.m_scale != nullptr) && small == (t.v_scale != nullptr), "adamw_update: tensor %d: scales come with 8-bit state", i);
+                    if (first) { master = t.master != nullptr; first = false; }
+                    PXE_REQUIRE(master == (t.master != nullptr), "adamw_update: a master copy in all tensors or in none");
+                    PXE_REQUIRE(!master || d.param_type != PXE_F32, "adamw_update: a master copy of fp32 parameters");
+                    PXE_REQUIRE(t.n <= (1LL << 40), "adamw_update: tensor %d has %lld elements", i, t.n);
+                    PXE_REQUIRE((uintptr_t)t.param % psize == 0 && (uintptr_t)t.grad % gsize == 0 && ((uintptr_t)t.m | (uintptr_t)t.v) % ssize == 0 &&
+                                ((uintptr_t)t.m_scale | (uintptr_t)t.v_scale | (uintptr_t)t.master) % 4 == 0,
+                                "adamw_update: tensor %d is not aligned to its elements", i);
+                }
+                const void* p[7] = {t.param, t.grad, t.m, t.v, t.m_scale, t.v_scale, t.master};
+                const long long bytes[7] = {t.n * psize, t.n * gsize, t.n * ssize, t.n * ssize, blocks * 4, blocks * 4, t.n * 4};
+                if (p[family]) ranges.push_back({(uintptr_t)p[family], (uintptr_t)p[family] + (uintptr_t)bytes[family], family != 1});
+            }
+        }
+        PXE_REQUIRE(!ranges_conflict(ranges), "adamw_update: tensors overlap (one listed twice, or a state, master or gradient inside another)");
+    } catch (const std::exception& e) {
+        return set_error(PXE_ERR_CUDA, "adamw_update: %s", e.what());
+    }
+    if (first) return PXE_OK;                              // nothing to do
+    DeviceInfo di;
+    { const int rc = device_info(&di); if (rc != PXE_OK) return rc; }
+    AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH> a;
+    a.rate = d.rate; a.b1 = d.beta1; a.b2 = d.beta2; a.omb1 = (float)(1.0 - (double)d.beta1); a.omb2 = (float)(1.0 - (double)d.beta2);
+    a.eps = d.eps; a.decay = d.weight_decay; a.grad_scale = d.grad_scale;
+    a.log_b1 = (float)std::log((double)d.beta1); a.log_b2 = (float)std::log((double)d.beta2);
+    a.inv_c1 = d.t_device ? 0.0f : (float)(1.0 / (1.0 - std::pow((double)d.beta1, (double)d.t)));
+    a.inv_c2 = d.t_device ? 0.0f : (float)(1.0 / (1.0 - std::pow((double)d.beta2, (double)d.t)));
+    a.rate_device = d.rate_device; a.t_device = d.t_device; a.grad_scale_device = d.grad_scale_device; a.skip_device = d.skip_device;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int i = 0;
+    while (i < d.count) {
+        a.count = 0;
+        long long chunks = 0;
+        for (; i < d.count && a.count < PXE_ADAMW_TENSORS_PER_LAUNCH; ++i) {
+            const pxe_adamw_tensor& t = d.tensors[i];
+            if (t.n == 0) continue;
+            const long long mine = (t.n + kChunk - 1) / kChunk;
+            if (chunks + mine > 0x3fffffffLL) break;       // chunk numbers are ints; n <= 2^40 leaves room for one tensor
+            Entry& e = a.e[a.count++];
+            e = {t.param, t.grad, t.m, t.v, t.m_scale, t.v_scale, t.master, t.n, (int)chunks, 0};
+            const int per = psize == 4 ? 4 : 8;            // elements per access
+            const uintptr_t wide = (uintptr_t)t.param | (uintptr_t)t.master | (small ? 0 : (uintptr_t)t.m | (uintptr_t)t.v);
+            e.vector = wide % 16 == 0 && (uintptr_t)t.grad % std::min(16, per * gsize) == 0 && (!small || ((uintptr_t)t.m | (uintptr_t)t.v) % per == 0);
+            chunks += mine;
+        }
+        if (a.count == 0) break;
+        a.chunks = (int)chunks;
+        int rc;
+        if (d.param_type == PXE_F32)
+            rc = d.grad_type == PXE_F32 ? launch<float, float>(s, a, di, small, master)
+               : d.grad_type == PXE_BF16 ? launch<float, bf16>(s, a, di, small, master) : launch<float, f16>(s, a, di, small, master);
+        else if (d.param_type == PXE_BF16)
+            rc = d.grad_type == PXE_F32 ? launch<bf16, float>(s, a, di, small, master) : launch<bf16, bf16>(s, a, di, small, master);
+        else
+            rc = d.grad_type == PXE_F32 ? launch<f16, float>(s, a, di, small, master) : launch<f16, f16>(s, a, di, small, master);
+        if (rc != PXE_OK) return rc;
+    }
+    return PXE_OK;
+}

@@ -8,7 +8,7 @@ how producers write straight into route (concat) buffers.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
@@ -822,3 +822,371 @@ def softmax_cross_entropy(pred: torch.Tensor, truth: torch.Tensor):
     capi.check(capi.lib().pxe_softmax_cross_entropy(_stream(), pred.numel(), pred.data_ptr(), truth.data_ptr(), delta.data_ptr(),
                                                     error.data_ptr()))
     return delta, error
+
+
+# ------------------------------------------------------------------------------ row operators in 32- and 16-bit types
+_DTYPE = {torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16}
+
+
+def _check_rows_cuda(t: torch.Tensor, name: str) -> int:
+    """The pxe_dtype of a float32, bfloat16 or float16 tensor on the current device."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPE):
+        raise TypeError(f"{name} must be a float32, bfloat16 or float16 CUDA tensor")
+    _check_device(t.device.index, name)
+    return _DTYPE[t.dtype]
+
+
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Distance in elements between consecutive rows of a [..., n] tensor whose rows are evenly spaced."""
+    shape, st = t.shape, t.stride()
+    n = shape[-1]
+    if t.numel() == 0:
+        return n
+    if n > 1 and st[-1] != 1:
+        raise ValueError(f"{name}: rows must be contiguous (strides {st} for shape {tuple(shape)})")
+    stride, span = None, 0                    # of the innermost dimension longer than 1; what the dimensions so far cover
+    for k in range(len(shape) - 2, -1, -1):
+        if shape[k] == 1:
+            continue
+        if stride is None:
+            stride, span = st[k], st[k] * shape[k]
+        elif st[k] != span:
+            raise ValueError(f"{name}: rows must be evenly spaced (strides {st} for shape {tuple(shape)})")
+        else:
+            span *= shape[k]
+    if stride is None:
+        return n
+    if stride < n:
+        raise ValueError(f"{name}: rows overlap (strides {st} for shape {tuple(shape)})")
+    return stride
+
+
+def _like(t: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise TypeError(f"{name} must be a CUDA tensor")
+    _check_device(t.device.index, name)
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, got {t.dtype} of {tuple(t.shape)}")
+    return t
+
+
+def _norm_weight(weight: Optional[torch.Tensor], x: torch.Tensor):
+    if weight is None:
+        return None, capi.F32
+    kind = _check_rows_cuda(weight, "weight")
+    if weight.dtype not in (torch.float32, x.dtype):
+        raise TypeError(f"weight must be float32 or {x.dtype}, got {weight.dtype}")
+    if weight.shape != x.shape[-1:] or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous tensor of {x.shape[-1]} elements")
+    return weight.data_ptr(), kind
+
+
+def _rms_norm(x, weight, residual, eps, residual_out):
+    """The part of the descriptor that both forms share, and (h, rstd)."""
+    d = capi.RmsNormDesc()
+    d.type = _check_rows_cuda(x, "x")
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] == 0:
+        raise ValueError(f"x must have channels, got shape {tuple(shape)}")
+    d.weight, d.weight_type = _norm_weight(weight, x)
+    d.channels, d.eps = shape[-1], eps
+    d.rows = rows = x.numel() // shape[-1]
+    d.x, d.x_row_stride = x.data_ptr(), _row_stride(x, "x")
+    h = x
+    if residual is not None:
+        _like(residual, shape, x.dtype, "residual")
+        h = torch.empty(shape, device=x.device, dtype=x.dtype) if residual_out is None else _like(residual_out, shape, x.dtype, "residual_out")
+        d.residual, d.residual_row_stride = residual.data_ptr(), _row_stride(residual, "residual")
+        d.h, d.h_row_stride = h.data_ptr(), _row_stride(h, "residual_out")
+    elif residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    rstd = torch.empty(shape[:-1], device=x.device, dtype=torch.float32)
+    d.rstd = rstd.data_ptr() if rows else None
+    return d, h, rstd
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
+             eps: float = 1e-6, out: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None):
+    """Root-mean-square norm over the last dimension, with the residual's addition in front:
+    ``h = x + residual``, ``y = h / sqrt(mean(h^2) + eps) * weight``.  Returns ``(y, h, rstd)``; ``h`` is ``x`` itself
+    without a residual, ``rstd`` (float32, one for each row) is what :func:`rms_norm_backward` needs.  ``x``: float32,
+    bfloat16 or float16 rows, evenly spaced (channels-last pixels: ``x.permute(0, 2, 3, 1)``); ``weight``: float32 or
+    x's type.  ``out`` and ``residual_out`` may be ``x`` or ``residual`` (not the same one)."""
+    d, h, rstd = _rms_norm(x, weight, residual, eps, residual_out)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out is None else _like(out, x.shape, x.dtype, "out")
+    d.y, d.y_row_stride = y.data_ptr(), _row_stride(y, "out")
+    if d.rows:
+        capi.check(capi.lib().pxe_rms_norm(_stream(), C.byref(d)))
+    return y, h, rstd
+
+
+def rms_norm_e4m3(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
+                  eps: float = 1e-6, group: int = 0, out: Optional[torch.Tensor] = None,
+                  residual_out: Optional[torch.Tensor] = None):
+    """:func:`rms_norm` with its result in 8 bits for a following product: returns ``(q, scale, h, rstd)`` with ``q``
+    float8_e4m3fn and ``y = q * scale``.  ``scale`` is float32 ``[..., ceil(channels / group)]``, one for every ``group``
+    (32, 64 or 128) channels of a row, or ``[..., 1]`` for the whole row with ``group=0``."""
+    if group not in (0, 32, 64, 128):
+        raise ValueError(f"group must be 0, 32, 64 or 128, got {group}")
+    d, h, rstd = _rms_norm(x, weight, residual, eps, residual_out)
+    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn) if out is None else _like(out, x.shape, torch.float8_e4m3fn, "out")
+    scale = torch.empty(x.shape[:-1] + (-(-d.channels // group) if group else 1,), device=x.device, dtype=torch.float32)
+    d.q, d.q_row_stride, d.scale, d.group = q.data_ptr(), _row_stride(q, "out"), scale.data_ptr(), group
+    if d.rows:
+        capi.check(capi.lib().pxe_rms_norm(_stream(), C.byref(d)))
+    return q, scale, h, rstd
+
+
+def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.Tensor], rstd: torch.Tensor, *,
+                      dresidual: Optional[torch.Tensor] = None, dweight: Optional[torch.Tensor] = None,
+                      dx: Optional[torch.Tensor] = None):
+    """Gradient of :func:`rms_norm`: returns ``(dx, dweight)``.  ``dx`` is the gradient of ``x`` and of the residual
+    alike; ``dresidual`` is the gradient that reaches ``h`` past the norm.  ``dweight`` (float32, ``None`` without a
+    weight) is added to when given, as :func:`batchnorm_backward` does, and made otherwise.  ``dx`` may be ``dy``,
+    ``h`` or ``dresidual``."""
+    d = capi.RmsNormBackwardDesc()
+    d.type = _check_rows_cuda(dy, "dy")
+    shape = dy.shape
+    if len(shape) == 0 or shape[-1] == 0:
+        raise ValueError(f"dy must have channels, got shape {tuple(shape)}")
+    _like(h, shape, dy.dtype, "h")
+    d.weight, d.weight_type = _norm_weight(weight, dy)
+    d.channels, d.rows = shape[-1], dy.numel() // shape[-1]
+    d.rstd = _vec(rstd, d.rows, "rstd")
+    d.dy, d.dy_row_stride = dy.data_ptr(), _row_stride(dy, "dy")
+    d.h, d.h_row_stride = h.data_ptr(), _row_stride(h, "h")
+    if dresidual is not None:
+        _like(dresidual, shape, dy.dtype, "dresidual")
+        d.dresidual, d.dresidual_row_stride = dresidual.data_ptr(), _row_stride(dresidual, "dresidual")
+    dx = torch.empty(shape, device=dy.device, dtype=dy.dtype) if dx is None else _like(dx, shape, dy.dtype, "dx")
+    d.dx, d.dx_row_stride = dx.data_ptr(), _row_stride(dx, "dx")
+    if dweight is not None:
+        d.dweight, d.accumulate = _vec(dweight, d.channels, "dweight"), 1
+    elif weight is not None:
+        dweight = torch.empty(d.channels, device=dy.device, dtype=torch.float32)
+        d.dweight = dweight.data_ptr()
+    if dweight is not None:
+        d.workspace_bytes = capi.lib().pxe_rms_norm_backward_workspace_bytes(d.rows, d.channels)
+        ws = torch.empty(d.workspace_bytes, device=dy.device, dtype=torch.uint8)
+        d.workspace = ws.data_ptr()
+    capi.check(capi.lib().pxe_rms_norm_backward(_stream(), C.byref(d)))
+    return dx, dweight
+
+
+class LogProbs(NamedTuple):
+    """What :func:`log_probs` returns; what was not asked for is None."""
+    logp: Optional[torch.Tensor]          # [...] float32
+    entropy: torch.Tensor                 # [...] float32
+    top_logp: Optional[torch.Tensor]      # [..., top] float32, largest first
+    top_index: Optional[torch.Tensor]     # [..., top] int32
+    stats: torch.Tensor                   # [..., 3] float32, for log_probs_backward
+
+
+def _grouped_rows(t: torch.Tensor, name: str):
+    """(inner, outer stride, row stride) of a [..., n] tensor: evenly spaced rows, or groups of them."""
+    if t.dim() > 2 and t.shape[0] > 1:
+        return t.numel() // (t.shape[0] * t.shape[-1]), t.stride(0), _row_stride(t[0], name)
+    return 0, 0, _row_stride(t, name)
+
+
+def _target(target: torch.Tensor, shape):
+    if not (isinstance(target, torch.Tensor) and target.is_cuda and target.dtype in (torch.int64, torch.int32)):
+        raise TypeError("target must be an int64 or int32 CUDA tensor")
+    _check_device(target.device.index, "target")
+    if target.shape != shape or not target.is_contiguous():
+        raise ValueError(f"target must be a contiguous tensor of shape {tuple(shape)}, got {tuple(target.shape)}")
+    return target.data_ptr(), int(target.dtype == torch.int64)
+
+
+def log_probs(x: torch.Tensor, target: Optional[torch.Tensor] = None, *, top: int = 0, temperature: float = 1.0) -> LogProbs:
+    """Log probabilities of given classes, the entropy and the ``top`` (up to 32) most likely classes of every row of
+    ``x`` [..., classes] (float32, bfloat16 or float16; a slice such as ``x[:, :-1]`` is read where it lies).  A negative
+    ``target`` marks a row that is not used: zeros, and -1 for its alternatives.  Ties go to the lower class."""
+    d = capi.LogProbsDesc()
+    d.type = _check_rows_cuda(x, "x")
+    shape, dev = x.shape, x.device
+    if len(shape) == 0 or shape[-1] == 0:
+        raise ValueError(f"x must have classes, got shape {tuple(shape)}")
+    d.classes, d.rows = shape[-1], x.numel() // shape[-1]
+    if not 0 <= top <= min(32, d.classes):
+        raise ValueError(f"top must lie in 0..{min(32, d.classes)}, got {top}")
+    d.top, d.temperature = top, temperature
+    shape = shape[:-1]
+    logp = top_logp = top_index = None
+    if target is not None:
+        d.target, d.target_is_int64 = _target(target, shape)
+        logp = torch.empty(shape, device=dev, dtype=torch.float32)
+        d.logp = logp.data_ptr()
+    entropy = torch.empty(shape, device=dev, dtype=torch.float32)
+    stats = torch.empty(shape + (3,), device=dev, dtype=torch.float32)
+    d.entropy, d.stats = entropy.data_ptr(), stats.data_ptr()
+    if top:
+        top_logp = torch.empty(shape + (top,), device=dev, dtype=torch.float32)
+        top_index = torch.empty(shape + (top,), device=dev, dtype=torch.int32)
+        d.top_logp, d.top_index = top_logp.data_ptr(), top_index.data_ptr()
+    if d.rows:
+        d.x = x.data_ptr()
+        d.inner, d.outer_stride, d.row_stride = _grouped_rows(x, "x")
+    capi.check(capi.lib().pxe_log_probs(_stream(), C.byref(d)))
+    return LogProbs(logp, entropy, top_logp, top_index, stats)
+
+
+def log_probs_backward(x: torch.Tensor, target: Optional[torch.Tensor], stats: torch.Tensor, dlogp: Optional[torch.Tensor] = None, *,
+                       dentropy: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                       dx: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of :func:`log_probs` with respect to ``x``, from the gradients of ``logp`` and of ``entropy`` (float32, one
+    for each row; either may be missing).  ``stats`` and ``temperature`` are the forward call's.  ``dx`` may be ``x``;
+    without it the gradient gets x's own strides."""
+    d = capi.LogProbsBackwardDesc()
+    d.type = _check_rows_cuda(x, "x")
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] == 0:
+        raise ValueError(f"x must have classes, got shape {tuple(shape)}")
+    d.classes, d.rows, d.temperature = shape[-1], x.numel() // shape[-1], temperature
+    d.stats = _vec(stats, 3 * d.rows, "stats")
+    if target is not None:
+        d.target, d.target_is_int64 = _target(target, shape[:-1])
+    d.dlogp, d.dentropy = _vec(dlogp, d.rows, "dlogp"), _vec(dentropy, d.rows, "dentropy")
+    if dlogp is not None and target is None:
+        raise ValueError("dlogp without target")
+    if dlogp is None and dentropy is None:
+        raise ValueError("neither dlogp nor dentropy")
+    if dx is None:
+        dx = torch.empty_strided(shape, x.stride(), device=x.device, dtype=x.dtype)
+    else:
+        _like(dx, shape, x.dtype, "dx")
+    if d.rows:
+        d.x, d.dx = x.data_ptr(), dx.data_ptr()
+        d.inner, d.outer_stride, d.row_stride = _grouped_rows(x, "x")
+        inner, d.dx_outer_stride, d.dx_row_stride = _grouped_rows(dx, "dx")
+    capi.check(capi.lib().pxe_log_probs_backward(_stream(), C.byref(d)))
+    return dx
+
+
+class AdamW:
+    """An AdamW step over many tensors at once (pxe_adamw_update), with its state.
+
+    ``params``: contiguous CUDA tensors of one type (float32, bfloat16 or float16) on one device.  ``state_bits=32``
+    keeps ``m`` and ``v`` as float32; ``state_bits=8`` keeps ``m`` and the root of ``v`` as float8_e4m3fn codes with a
+    float32 scale for every 256 elements (``m_scale``, ``v_scale``).  ``master=True`` keeps float32 copies of 16-bit
+    parameters and updates those.  All are lists, one tensor for each parameter; lists of an earlier state can be given
+    instead (a loaded checkpoint) and are then updated in place.  The plan holds the parameters; one whose memory
+    has moved since is refused by :meth:`step`."""
+
+    def __init__(self, params: Sequence[torch.Tensor], *, state_bits: int = 32, m=None, v=None, m_scale=None, v_scale=None, master=None):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        self.params = list(params)
+        self.state_bits = state_bits
+        self._dtype, self._device = torch.float32, None
+        for i, p in enumerate(self.params):
+            _check_rows_cuda(p, f"params[{i}]")
+            if i == 0:
+                self._dtype, self._device = p.dtype, p.device
+            if p.dtype != self._dtype:
+                raise TypeError(f"params[{i}] is {p.dtype}, the others {self._dtype}: one plan for each type")
+            if not p.is_contiguous():
+                raise ValueError(f"params[{i}] must be contiguous")
+        self._sizes = [p.numel() for p in self.params]
+        self._shapes = [p.shape for p in self.params]
+        blocks = [-(-n // capi.ADAMW_BLOCK) for n in self._sizes]
+        small = state_bits == 8
+        if (m is None) != (v is None) or (not small and (m_scale is not None or v_scale is not None)) \
+                or (small and not ((m is None) == (m_scale is None) == (v_scale is None))):
+            raise ValueError("an earlier state is m and v, and m_scale and v_scale with 8 bits")
+        state = torch.float8_e4m3fn if small else torch.float32
+        self.m, self.v = (self._state(t, self._sizes, state, n) for t, n in ((m, "m"), (v, "v")))
+        self.m_scale, self.v_scale = ((self._state(t, blocks, torch.float32, n) for t, n in ((m_scale, "m_scale"), (v_scale, "v_scale")))
+                                      if small else (None, None))
+        self.master = None
+        if master is not None and master is not False:
+            if self._dtype == torch.float32:
+                raise ValueError("a master copy of float32 parameters")
+            self.master = self._state(None if master is True else master, self._sizes, torch.float32, "master")
+            if master is True:
+                for w, p in zip(self.master, self.params):
+                    w.copy_(p.detach().reshape(-1))
+        count = len(self.params)
+        self._table = (capi.AdamwTensor * max(count, 1))()
+        self._ptrs = [p.data_ptr() for p in self.params]
+        for i, row in enumerate(self._table[:count]):
+            row.param, row.n = self._ptrs[i], self._sizes[i]
+            row.m, row.v = self.m[i].data_ptr(), self.v[i].data_ptr()
+            if small:
+                row.m_scale, row.v_scale = self.m_scale[i].data_ptr(), self.v_scale[i].data_ptr()
+            if self.master is not None:
+                row.master = self.master[i].data_ptr()
+        # the addresses of the gradients, as a column of the table
+        self._grads = np.frombuffer(self._table, dtype=np.uint64).reshape(-1, C.sizeof(capi.AdamwTensor) // 8)[:count, capi.AdamwTensor.grad.offset // 8]
+        d = self._desc = capi.AdamwDesc()
+        d.tensors, d.count, d.state_bits, d.param_type = C.addressof(self._table), count, state_bits, _DTYPE[self._dtype]
+
+    def _state(self, given, sizes, dtype, name):
+        if given is None:                    # one buffer, every tensor on a 256-byte boundary
+            unit = 256 // dtype.itemsize
+            at = [0]
+            for n in sizes:
+                at.append(at[-1] + -(-n // unit) * unit)
+            buf = torch.zeros(at[-1], device=self._device, dtype=torch.float32 if dtype == torch.float32 else torch.uint8).view(dtype)
+            return [buf[o:o + n] for o, n in zip(at, sizes)]
+        given = list(given)
+        if len(given) != len(sizes):
+            raise ValueError(f"{name} has {len(given)} tensors for {len(sizes)} parameters")
+        for i, (t, n) in enumerate(zip(given, sizes)):
+            if not t.is_cuda or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"{name}[{i}] must be a contiguous {dtype} CUDA tensor of {n} elements")
+            _check_device(t.device.index, f"{name}[{i}]")
+        return given
+
+    def _scalar(self, t, dtype, name):
+        if not t.is_cuda or t.dtype != dtype or t.numel() != 1:
+            raise TypeError(f"{name} must be a number or a {dtype} CUDA tensor of one element")
+        _check_device(t.device.index, name)
+        return t.data_ptr()
+
+    def step(self, grads: Sequence[torch.Tensor], *, rate, t, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
+             weight_decay: float = 0.0, grad_scale=1.0, skip: Optional[torch.Tensor] = None) -> None:
+        """One step, in place on the parameters and the state.  ``grads``: one contiguous tensor for each parameter, all
+        of one type (float32 or the parameters' own; any of the three types for float32 parameters).  ``t`` counts steps
+        from 1.  ``rate``, ``grad_scale`` (float32) and ``t`` (int64) may be CUDA tensors of one element, which a captured
+        step reads at every replay; ``skip``: a float32 one that, not 0, makes the step do nothing."""
+        params = self.params
+        count = len(params)
+        if len(grads) != count:
+            raise ValueError(f"{len(grads)} gradients for {count} parameters")
+        if count == 0:
+            return
+        _check_device(self._device.index, "params")
+        if [p.data_ptr() for p in params] != self._ptrs:
+            raise RuntimeError("a parameter's memory has moved since this plan was made; make a new one")
+        kind, device = getattr(grads[0], "dtype", None), self._device
+        if kind not in _DTYPE:
+            raise TypeError(f"gradients must be float32, bfloat16 or float16 tensors, got {kind}")
+        ptrs = []
+        for i, (g, shape) in enumerate(zip(grads, self._shapes)):
+            if not isinstance(g, torch.Tensor):
+                raise TypeError(f"grads[{i}] is not a tensor")
+            if g.dtype is not kind or g.shape != shape or g.device != device or not g.is_contiguous():
+                raise ValueError(f"gradients must be contiguous {kind} tensors on {device} of the parameters' shapes; "
+                                 f"got {g.dtype} on {g.device} of shape {tuple(g.shape)} for {tuple(shape)}")
+            ptrs.append(g.data_ptr())
+        self._grads[:] = ptrs
+        d = self._desc
+        d.grad_type = _DTYPE[kind]
+        d.rate_device = d.t_device = d.grad_scale_device = d.skip_device = None
+        if isinstance(rate, torch.Tensor):
+            d.rate_device = self._scalar(rate, torch.float32, "rate")
+        else:
+            d.rate = rate
+        if isinstance(t, torch.Tensor):
+            d.t_device = self._scalar(t, torch.int64, "t")
+        else:
+            d.t = t
+        if isinstance(grad_scale, torch.Tensor):
+            d.grad_scale_device = self._scalar(grad_scale, torch.float32, "grad_scale")
+        else:
+            d.grad_scale = grad_scale
+        if skip is not None:
+            d.skip_device = self._scalar(skip, torch.float32, "skip")
+        d.beta1, d.beta2, d.eps, d.weight_decay = beta1, beta2, eps, weight_decay
+        capi.check(capi.lib().pxe_adamw_update(_stream(), C.byref(d)))

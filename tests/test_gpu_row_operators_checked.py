@@ -1,0 +1,24 @@
+"""The row operators' suite once more on the bounds-checked build of the library (see test_gpu_bounds_checked.py): an access
+of one of their kernels outside the live allocations fails the test that made it.  The longest rows are left out (every
+access is a search), and what is captured into a graph, since a table cannot be installed during a capture."""
+import os
+import re
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.gpu
+def test_row_operators_on_the_bounds_checked_build(cuda):
+    env = dict(os.environ, PXE_TEST_BOUNDS_CHECKED="1")
+    cmd = [sys.executable, "-m", "pytest", "-q", "-x", "-m", "gpu", "-p", "no:cacheprovider", "-k",
+           "not graph and not served and not streams and not many_large and not 70000 and not shape12 and not shape11",
+           os.path.join("tests", "test_gpu_row_operators.py")]
+    res = subprocess.run(cmd, cwd=ROOT, env=env, capture_output=True, text=True, timeout=1500)
+    tail = res.stdout[-3000:] + res.stderr[-2000:]
+    assert res.returncode == 0, tail
+    m = re.search(r"(\d+) passed", res.stdout)
+    assert m and int(m.group(1)) >= 400, tail
