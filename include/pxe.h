@@ -685,7 +685,7 @@ PXE_API int pxe_rms_norm_backward(pxe_stream_t stream, const pxe_rms_norm_backwa
  *   logp = d_target - log S,  entropy = log S - sum(exp(d_j) * d_j) / S,
  *   top_index / top_logp: the `top` largest values, largest first, ties to the lower class.
  * Row r lies at x + (r / inner) * outer_stride + (r % inner) * row_stride, so that a slice of a [batch, length, classes]
- * tensor needs no copy.  A row with target < 0 is not used: it is not read, its logp, entropy and top_logp are 0, its
+ * tensor needs no copy.  A row with target < 0 is not used: whatever it holds, its logp, entropy and top_logp are 0, its
  * top_index -1.  A target >= classes gives a logp of NaN (nothing is read there).  Values of -inf have probability 0; a row
  * of nothing else has logp -inf and entropy 0.  A row with a NaN or +inf has logp and entropy NaN; a NaN counts as
  * larger than every number among the alternatives.  rows == 0: nothing to do. */
@@ -702,7 +702,7 @@ typedef struct pxe_log_probs_desc {
     int type;                  /* enum pxe_dtype of x */
     int target_is_int64;
     int top;                   /* 0..32, at most classes */
-    float temperature;         /* > 0 */
+    float temperature;         /* 1e-30 .. 1e30 */
 } pxe_log_probs_desc;
 PXE_API int pxe_log_probs(pxe_stream_t stream, const pxe_log_probs_desc* desc);
 

@@ -38,12 +38,32 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ f16 from_f32<f16>(float v) { return __float2half_rn(v); }
 
+// the two elements of a word
+template <typename T> __device__ __forceinline__ void split(uint32_t w, float& x, float& y);
+template <> __device__ __forceinline__ void split<bf16>(uint32_t w, float& x, float& y)
+{
+    x = __uint_as_float(w << 16);                          // a bf16 is the upper half of its float
+    y = __uint_as_float(w & 0xffff0000u);
+}
+template <> __device__ __forceinline__ void split<f16>(uint32_t w, float& x, float& y)
+{
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    x = f.x;
+    y = f.y;
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void unpack(const Raw<T, N>& raw, float (&f)[N])
 {
-    const T* e = reinterpret_cast<const T*>(&raw);
+    if constexpr (sizeof(T) == 2 && N >= 2) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = to_f32<T>(e[i]);
+        for (int i = 0; i < N / 2; ++i) split<T>(w[i], f[2 * i], f[2 * i + 1]);
+    } else {
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = to_f32<T>(e[i]);
+    }
 }
 template <typename T, int N>
 __device__ __forceinline__ Raw<T, N> pack(const float (&f)[N])
@@ -100,11 +120,43 @@ __device__ __forceinline__ void unpack_e4m3(const typename RawOf<N>::type& raw, 
     }
 }
 
+// The scale of values up to `largest` and its reciprocal (the scale is a normal number, so that neither overflows).
+__device__ __forceinline__ float max_nan(float a, float b);
+__device__ __forceinline__ float e4m3_scale(float largest) { return max_nan(largest * (1.0f / kE4m3Max), kScaleMin); }
+__device__ __forceinline__ float e4m3_inverse(float scale) { return fast_rcp(scale); }
+
 // max that keeps a NaN (fmaxf drops it)
 __device__ __forceinline__ float max_nan(float a, float b)
 {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// ---------------------------------------------------------------- two floats an instruction
+__device__ __forceinline__ unsigned long long pair(float a, float b)
+{
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(unsigned long long p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c)
+{
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b)
+{
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b)
+{
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 

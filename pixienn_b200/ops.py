@@ -825,23 +825,50 @@ def softmax_cross_entropy(pred: torch.Tensor, truth: torch.Tensor):
 
 
 # ------------------------------------------------------------------------------ row operators in 32- and 16-bit types
+# A call on a token's row is as long as its marshalling, so these read each property of a tensor once and fill their
+# descriptors in one go.
 _DTYPE = {torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16}
+_raw_stream = torch._C._cuda_getCurrentRawStream          # of a device's index; what current_stream(...).cuda_stream reads
 
 
-def _check_rows_cuda(t: torch.Tensor, name: str) -> int:
-    """The pxe_dtype of a float32, bfloat16 or float16 tensor on the current device."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPE):
+def _new(shape, dtype, device) -> torch.Tensor:
+    """A dense tensor; empty_strided is the cheapest of torch's ways to make one."""
+    n = len(shape)
+    if n == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    if n == 2:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _rows_device(t: torch.Tensor, name: str) -> int:
+    """Index of the current device, which a float32, bfloat16 or float16 CUDA tensor has to live on."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPE or not t.is_cuda:
         raise TypeError(f"{name} must be a float32, bfloat16 or float16 CUDA tensor")
-    _check_device(t.device.index, name)
-    return _DTYPE[t.dtype]
+    dev = t.get_device()
+    if dev != torch.cuda.current_device():
+        _check_device(dev, name)
+    return dev
+
+
+def _like(t: torch.Tensor, shape, dtype, dev: int, name: str) -> torch.Tensor:
+    """t, a tensor of this shape and type on device `dev`."""
+    if not isinstance(t, torch.Tensor) or t.get_device() < 0:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.get_device() != dev:
+        _check_device(t.get_device(), name)
+    if t.shape != shape or t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, got {t.dtype} of {tuple(t.shape)}")
+    return t
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
     """Distance in elements between consecutive rows of a [..., n] tensor whose rows are evenly spaced."""
-    shape, st = t.shape, t.stride()
+    return t.shape[-1] if t.is_contiguous() else _even_stride(t.shape, t.stride(), name)
+
+
+def _even_stride(shape, st, name: str) -> int:
     n = shape[-1]
-    if t.numel() == 0:
-        return n
     if n > 1 and st[-1] != 1:
         raise ValueError(f"{name}: rows must be contiguous (strides {st} for shape {tuple(shape)})")
     stride, span = None, 0                    # of the innermost dimension longer than 1; what the dimensions so far cover
@@ -861,48 +888,62 @@ def _row_stride(t: torch.Tensor, name: str) -> int:
     return stride
 
 
-def _like(t: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        raise TypeError(f"{name} must be a CUDA tensor")
-    _check_device(t.device.index, name)
-    if t.shape != shape or t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, got {t.dtype} of {tuple(t.shape)}")
-    return t
+def _dense_f32(t: Optional[torch.Tensor], n: int, dev: int, name: str):
+    """Address of a contiguous float32 tensor of n elements."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.get_device() != dev:
+        _check_f32_cuda(t, name)
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of {n} elements")
+    return t.data_ptr()
 
 
-def _norm_weight(weight: Optional[torch.Tensor], x: torch.Tensor):
-    if weight is None:
-        return None, capi.F32
-    kind = _check_rows_cuda(weight, "weight")
-    if weight.dtype not in (torch.float32, x.dtype):
-        raise TypeError(f"weight must be float32 or {x.dtype}, got {weight.dtype}")
-    if weight.shape != x.shape[-1:] or not weight.is_contiguous():
-        raise ValueError(f"weight must be a contiguous tensor of {x.shape[-1]} elements")
-    return weight.data_ptr(), kind
-
-
-def _rms_norm(x, weight, residual, eps, residual_out):
-    """The part of the descriptor that both forms share, and (h, rstd)."""
-    d = capi.RmsNormDesc()
-    d.type = _check_rows_cuda(x, "x")
+def _channels(x: torch.Tensor, name: str, what: str = "channels") -> int:
     shape = x.shape
     if len(shape) == 0 or shape[-1] == 0:
-        raise ValueError(f"x must have channels, got shape {tuple(shape)}")
-    d.weight, d.weight_type = _norm_weight(weight, x)
-    d.channels, d.eps = shape[-1], eps
-    d.rows = rows = x.numel() // shape[-1]
-    d.x, d.x_row_stride = x.data_ptr(), _row_stride(x, "x")
-    h = x
+        raise ValueError(f"{name} must have {what}, got shape {tuple(shape)}")
+    return shape[-1]
+
+
+def _norm_weight(weight: Optional[torch.Tensor], channels: int, dtype, dev: int):
+    if weight is None:
+        return None, capi.F32
+    if not isinstance(weight, torch.Tensor) or weight.get_device() != dev:
+        _rows_device(weight, "weight")
+    if weight.dtype is not torch.float32 and weight.dtype is not dtype:
+        raise TypeError(f"weight must be float32 or {dtype}, got {weight.dtype}")
+    if weight.dim() != 1 or weight.numel() != channels or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous tensor of {channels} elements")
+    return weight.data_ptr(), _DTYPE[weight.dtype]
+
+
+def _rms_norm(x, weight, residual, eps, out, residual_out, e4m3, group):
+    dev = _rows_device(x, "x")
+    channels, dtype, shape = _channels(x, "x"), x.dtype, x.shape
+    wp, wtype = _norm_weight(weight, channels, dtype, dev)
+    rows = x.numel() // channels
+    h, rp, rs, hp, hs = x, None, 0, None, 0
     if residual is not None:
-        _like(residual, shape, x.dtype, "residual")
-        h = torch.empty(shape, device=x.device, dtype=x.dtype) if residual_out is None else _like(residual_out, shape, x.dtype, "residual_out")
-        d.residual, d.residual_row_stride = residual.data_ptr(), _row_stride(residual, "residual")
-        d.h, d.h_row_stride = h.data_ptr(), _row_stride(h, "residual_out")
+        _like(residual, shape, dtype, dev, "residual")
+        rp, rs = residual.data_ptr(), _row_stride(residual, "residual")
+        h = torch.empty_like(x) if residual_out is None else _like(residual_out, shape, dtype, dev, "residual_out")
+        hp, hs = h.data_ptr(), _row_stride(h, "residual_out")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    rstd = torch.empty(shape[:-1], device=x.device, dtype=torch.float32)
-    d.rstd = rstd.data_ptr() if rows else None
-    return d, h, rstd
+    rstd = _new(shape[:-1], torch.float32, x.device)
+    kind = torch.float8_e4m3fn if e4m3 else dtype
+    y = torch.empty_like(x, dtype=kind) if out is None else _like(out, shape, kind, dev, "out")
+    yp, ys, scale, sp = y.data_ptr(), _row_stride(y, "out"), None, None
+    if e4m3:
+        scale = _new(shape[:-1] + (-(-channels // group) if group else 1,), torch.float32, x.device)
+        sp = scale.data_ptr()
+    if rows:
+        d = capi.RmsNormDesc(x.data_ptr(), rp, wp, hp, None if e4m3 else yp, yp if e4m3 else None, sp, rstd.data_ptr(),
+                             _row_stride(x, "x"), rs, hs, 0 if e4m3 else ys, ys if e4m3 else 0, rows, channels, _DTYPE[dtype], wtype,
+                             group, eps)
+        capi.check(capi.lib().pxe_rms_norm(_raw_stream(dev), C.byref(d)))
+    return y, scale, h, rstd
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
@@ -912,11 +953,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     without a residual, ``rstd`` (float32, one for each row) is what :func:`rms_norm_backward` needs.  ``x``: float32,
     bfloat16 or float16 rows, evenly spaced (channels-last pixels: ``x.permute(0, 2, 3, 1)``); ``weight``: float32 or
     x's type.  ``out`` and ``residual_out`` may be ``x`` or ``residual`` (not the same one)."""
-    d, h, rstd = _rms_norm(x, weight, residual, eps, residual_out)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out is None else _like(out, x.shape, x.dtype, "out")
-    d.y, d.y_row_stride = y.data_ptr(), _row_stride(y, "out")
-    if d.rows:
-        capi.check(capi.lib().pxe_rms_norm(_stream(), C.byref(d)))
+    y, _, h, rstd = _rms_norm(x, weight, residual, eps, out, residual_out, False, 0)
     return y, h, rstd
 
 
@@ -928,13 +965,7 @@ def rms_norm_e4m3(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, res
     (32, 64 or 128) channels of a row, or ``[..., 1]`` for the whole row with ``group=0``."""
     if group not in (0, 32, 64, 128):
         raise ValueError(f"group must be 0, 32, 64 or 128, got {group}")
-    d, h, rstd = _rms_norm(x, weight, residual, eps, residual_out)
-    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn) if out is None else _like(out, x.shape, torch.float8_e4m3fn, "out")
-    scale = torch.empty(x.shape[:-1] + (-(-d.channels // group) if group else 1,), device=x.device, dtype=torch.float32)
-    d.q, d.q_row_stride, d.scale, d.group = q.data_ptr(), _row_stride(q, "out"), scale.data_ptr(), group
-    if d.rows:
-        capi.check(capi.lib().pxe_rms_norm(_stream(), C.byref(d)))
-    return q, scale, h, rstd
+    return _rms_norm(x, weight, residual, eps, out, residual_out, True, group)
 
 
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.Tensor], rstd: torch.Tensor, *,
@@ -944,32 +975,30 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.
     alike; ``dresidual`` is the gradient that reaches ``h`` past the norm.  ``dweight`` (float32, ``None`` without a
     weight) is added to when given, as :func:`batchnorm_backward` does, and made otherwise.  ``dx`` may be ``dy``,
     ``h`` or ``dresidual``."""
-    d = capi.RmsNormBackwardDesc()
-    d.type = _check_rows_cuda(dy, "dy")
-    shape = dy.shape
-    if len(shape) == 0 or shape[-1] == 0:
-        raise ValueError(f"dy must have channels, got shape {tuple(shape)}")
-    _like(h, shape, dy.dtype, "h")
-    d.weight, d.weight_type = _norm_weight(weight, dy)
-    d.channels, d.rows = shape[-1], dy.numel() // shape[-1]
-    d.rstd = _vec(rstd, d.rows, "rstd")
-    d.dy, d.dy_row_stride = dy.data_ptr(), _row_stride(dy, "dy")
-    d.h, d.h_row_stride = h.data_ptr(), _row_stride(h, "h")
+    dev = _rows_device(dy, "dy")
+    channels, dtype, shape = _channels(dy, "dy"), dy.dtype, dy.shape
+    rows = dy.numel() // channels
+    _like(h, shape, dtype, dev, "h")
+    wp, wtype = _norm_weight(weight, channels, dtype, dev)
+    rp, rs = None, 0
     if dresidual is not None:
-        _like(dresidual, shape, dy.dtype, "dresidual")
-        d.dresidual, d.dresidual_row_stride = dresidual.data_ptr(), _row_stride(dresidual, "dresidual")
-    dx = torch.empty(shape, device=dy.device, dtype=dy.dtype) if dx is None else _like(dx, shape, dy.dtype, "dx")
-    d.dx, d.dx_row_stride = dx.data_ptr(), _row_stride(dx, "dx")
+        _like(dresidual, shape, dtype, dev, "dresidual")
+        rp, rs = dresidual.data_ptr(), _row_stride(dresidual, "dresidual")
+    dx = torch.empty_like(dy) if dx is None else _like(dx, shape, dtype, dev, "dx")
+    accumulate, ws, wsp, nbytes, dwp = 0, None, None, 0, None
     if dweight is not None:
-        d.dweight, d.accumulate = _vec(dweight, d.channels, "dweight"), 1
+        dwp, accumulate = _dense_f32(dweight, channels, dev, "dweight"), 1
     elif weight is not None:
-        dweight = torch.empty(d.channels, device=dy.device, dtype=torch.float32)
-        d.dweight = dweight.data_ptr()
-    if dweight is not None:
-        d.workspace_bytes = capi.lib().pxe_rms_norm_backward_workspace_bytes(d.rows, d.channels)
-        ws = torch.empty(d.workspace_bytes, device=dy.device, dtype=torch.uint8)
-        d.workspace = ws.data_ptr()
-    capi.check(capi.lib().pxe_rms_norm_backward(_stream(), C.byref(d)))
+        dweight = _new((channels,), torch.float32, dy.device)
+        dwp = dweight.data_ptr()
+    if dwp is not None:
+        nbytes = capi.lib().pxe_rms_norm_backward_workspace_bytes(rows, channels)
+        ws = _new((nbytes,), torch.uint8, dy.device)
+        wsp = ws.data_ptr()
+    d = capi.RmsNormBackwardDesc(dy.data_ptr(), h.data_ptr(), rp, wp, _dense_f32(rstd, rows, dev, "rstd"), dx.data_ptr(), dwp,
+                                 _row_stride(dy, "dy"), _row_stride(h, "h"), rs, _row_stride(dx, "dx"), rows, channels, _DTYPE[dtype],
+                                 wtype, accumulate, wsp, nbytes)
+    capi.check(capi.lib().pxe_rms_norm_backward(_raw_stream(dev), C.byref(d)))
     return dx, dweight
 
 
@@ -984,50 +1013,47 @@ class LogProbs(NamedTuple):
 
 def _grouped_rows(t: torch.Tensor, name: str):
     """(inner, outer stride, row stride) of a [..., n] tensor: evenly spaced rows, or groups of them."""
-    if t.dim() > 2 and t.shape[0] > 1:
-        return t.numel() // (t.shape[0] * t.shape[-1]), t.stride(0), _row_stride(t[0], name)
+    shape = t.shape
+    if len(shape) > 2 and shape[0] > 1 and t.numel():
+        st = t.stride()
+        return t.numel() // (shape[0] * shape[-1]), st[0], _even_stride(shape[1:], st[1:], name)
     return 0, 0, _row_stride(t, name)
 
 
-def _target(target: torch.Tensor, shape):
-    if not (isinstance(target, torch.Tensor) and target.is_cuda and target.dtype in (torch.int64, torch.int32)):
+def _target(target: torch.Tensor, shape, dev: int):
+    if not isinstance(target, torch.Tensor) or target.dtype not in (torch.int64, torch.int32) or not target.is_cuda:
         raise TypeError("target must be an int64 or int32 CUDA tensor")
-    _check_device(target.device.index, "target")
+    if target.get_device() != dev:
+        _check_device(target.get_device(), "target")
     if target.shape != shape or not target.is_contiguous():
         raise ValueError(f"target must be a contiguous tensor of shape {tuple(shape)}, got {tuple(target.shape)}")
-    return target.data_ptr(), int(target.dtype == torch.int64)
+    return target.data_ptr(), int(target.dtype is torch.int64)
 
 
 def log_probs(x: torch.Tensor, target: Optional[torch.Tensor] = None, *, top: int = 0, temperature: float = 1.0) -> LogProbs:
     """Log probabilities of given classes, the entropy and the ``top`` (up to 32) most likely classes of every row of
     ``x`` [..., classes] (float32, bfloat16 or float16; a slice such as ``x[:, :-1]`` is read where it lies).  A negative
     ``target`` marks a row that is not used: zeros, and -1 for its alternatives.  Ties go to the lower class."""
-    d = capi.LogProbsDesc()
-    d.type = _check_rows_cuda(x, "x")
-    shape, dev = x.shape, x.device
-    if len(shape) == 0 or shape[-1] == 0:
-        raise ValueError(f"x must have classes, got shape {tuple(shape)}")
-    d.classes, d.rows = shape[-1], x.numel() // shape[-1]
-    if not 0 <= top <= min(32, d.classes):
-        raise ValueError(f"top must lie in 0..{min(32, d.classes)}, got {top}")
-    d.top, d.temperature = top, temperature
-    shape = shape[:-1]
-    logp = top_logp = top_index = None
+    dev = _rows_device(x, "x")
+    classes, shape = _channels(x, "x", "classes"), x.shape[:-1]
+    rows = x.numel() // classes
+    if not 0 <= top <= min(32, classes):
+        raise ValueError(f"top must lie in 0..{min(32, classes)}, got {top}")
+    f32 = torch.float32
+    logp = top_logp = top_index = tp = lp = vp = ip = None
+    is64 = 0
     if target is not None:
-        d.target, d.target_is_int64 = _target(target, shape)
-        logp = torch.empty(shape, device=dev, dtype=torch.float32)
-        d.logp = logp.data_ptr()
-    entropy = torch.empty(shape, device=dev, dtype=torch.float32)
-    stats = torch.empty(shape + (3,), device=dev, dtype=torch.float32)
-    d.entropy, d.stats = entropy.data_ptr(), stats.data_ptr()
+        tp, is64 = _target(target, shape, dev)
+        logp = _new(shape, f32, x.device)
+        lp = logp.data_ptr()
+    entropy, stats = _new(shape, f32, x.device), _new(shape + (3,), f32, x.device)
     if top:
-        top_logp = torch.empty(shape + (top,), device=dev, dtype=torch.float32)
-        top_index = torch.empty(shape + (top,), device=dev, dtype=torch.int32)
-        d.top_logp, d.top_index = top_logp.data_ptr(), top_index.data_ptr()
-    if d.rows:
-        d.x = x.data_ptr()
-        d.inner, d.outer_stride, d.row_stride = _grouped_rows(x, "x")
-    capi.check(capi.lib().pxe_log_probs(_stream(), C.byref(d)))
+        top_logp, top_index = _new(shape + (top,), f32, x.device), _new(shape + (top,), torch.int32, x.device)
+        vp, ip = top_logp.data_ptr(), top_index.data_ptr()
+    inner, outer, stride = _grouped_rows(x, "x")
+    d = capi.LogProbsDesc(x.data_ptr(), tp, lp, entropy.data_ptr(), stats.data_ptr(), vp, ip, rows, inner, outer, stride, classes,
+                          _DTYPE[x.dtype], is64, top, temperature)
+    capi.check(capi.lib().pxe_log_probs(_raw_stream(dev), C.byref(d)))
     return LogProbs(logp, entropy, top_logp, top_index, stats)
 
 
@@ -1037,29 +1063,24 @@ def log_probs_backward(x: torch.Tensor, target: Optional[torch.Tensor], stats: t
     """Gradient of :func:`log_probs` with respect to ``x``, from the gradients of ``logp`` and of ``entropy`` (float32, one
     for each row; either may be missing).  ``stats`` and ``temperature`` are the forward call's.  ``dx`` may be ``x``;
     without it the gradient gets x's own strides."""
-    d = capi.LogProbsBackwardDesc()
-    d.type = _check_rows_cuda(x, "x")
-    shape = x.shape
-    if len(shape) == 0 or shape[-1] == 0:
-        raise ValueError(f"x must have classes, got shape {tuple(shape)}")
-    d.classes, d.rows, d.temperature = shape[-1], x.numel() // shape[-1], temperature
-    d.stats = _vec(stats, 3 * d.rows, "stats")
-    if target is not None:
-        d.target, d.target_is_int64 = _target(target, shape[:-1])
-    d.dlogp, d.dentropy = _vec(dlogp, d.rows, "dlogp"), _vec(dentropy, d.rows, "dentropy")
-    if dlogp is not None and target is None:
-        raise ValueError("dlogp without target")
+    dev = _rows_device(x, "x")
+    classes, shape = _channels(x, "x", "classes"), x.shape
+    rows = x.numel() // classes
     if dlogp is None and dentropy is None:
         raise ValueError("neither dlogp nor dentropy")
+    if dlogp is not None and target is None:
+        raise ValueError("dlogp without target")
+    tp, is64 = _target(target, shape[:-1], dev) if target is not None else (None, 0)
+    inner, outer, stride = _grouped_rows(x, "x")
     if dx is None:
         dx = torch.empty_strided(shape, x.stride(), device=x.device, dtype=x.dtype)
+        dx_outer, dx_stride = outer, stride
     else:
-        _like(dx, shape, x.dtype, "dx")
-    if d.rows:
-        d.x, d.dx = x.data_ptr(), dx.data_ptr()
-        d.inner, d.outer_stride, d.row_stride = _grouped_rows(x, "x")
-        inner, d.dx_outer_stride, d.dx_row_stride = _grouped_rows(dx, "dx")
-    capi.check(capi.lib().pxe_log_probs_backward(_stream(), C.byref(d)))
+        _, dx_outer, dx_stride = _grouped_rows(_like(dx, shape, x.dtype, dev, "dx"), "dx")
+    d = capi.LogProbsBackwardDesc(x.data_ptr(), tp, _dense_f32(stats, 3 * rows, dev, "stats"), _dense_f32(dlogp, rows, dev, "dlogp"),
+                                  _dense_f32(dentropy, rows, dev, "dentropy"), dx.data_ptr(), rows, inner, outer, stride, dx_outer,
+                                  dx_stride, classes, _DTYPE[x.dtype], is64, temperature)
+    capi.check(capi.lib().pxe_log_probs_backward(_raw_stream(dev), C.byref(d)))
     return dx
 
 
@@ -1080,7 +1101,7 @@ class AdamW:
         self.state_bits = state_bits
         self._dtype, self._device = torch.float32, None
         for i, p in enumerate(self.params):
-            _check_rows_cuda(p, f"params[{i}]")
+            _rows_device(p, f"params[{i}]")
             if i == 0:
                 self._dtype, self._device = p.dtype, p.device
             if p.dtype != self._dtype:
@@ -1156,18 +1177,20 @@ class AdamW:
             raise ValueError(f"{len(grads)} gradients for {count} parameters")
         if count == 0:
             return
-        _check_device(self._device.index, "params")
+        dev = self._device.index
+        if dev != torch.cuda.current_device():
+            _check_device(dev, "params")
         if [p.data_ptr() for p in params] != self._ptrs:
             raise RuntimeError("a parameter's memory has moved since this plan was made; make a new one")
-        kind, device = getattr(grads[0], "dtype", None), self._device
+        kind = getattr(grads[0], "dtype", None)
         if kind not in _DTYPE:
             raise TypeError(f"gradients must be float32, bfloat16 or float16 tensors, got {kind}")
         ptrs = []
         for i, (g, shape) in enumerate(zip(grads, self._shapes)):
             if not isinstance(g, torch.Tensor):
                 raise TypeError(f"grads[{i}] is not a tensor")
-            if g.dtype is not kind or g.shape != shape or g.device != device or not g.is_contiguous():
-                raise ValueError(f"gradients must be contiguous {kind} tensors on {device} of the parameters' shapes; "
+            if g.dtype is not kind or g.shape != shape or g.get_device() != dev or not g.is_contiguous():
+                raise ValueError(f"gradients must be contiguous {kind} tensors on {self._device} of the parameters' shapes; "
                                  f"got {g.dtype} on {g.device} of shape {tuple(g.shape)} for {tuple(shape)}")
             ptrs.append(g.data_ptr())
         self._grads[:] = ptrs
@@ -1189,4 +1212,4 @@ class AdamW:
         if skip is not None:
             d.skip_device = self._scalar(skip, torch.float32, "skip")
         d.beta1, d.beta2, d.eps, d.weight_decay = beta1, beta2, eps, weight_decay
-        capi.check(capi.lib().pxe_adamw_update(_stream(), C.byref(d)))
+        capi.check(capi.lib().pxe_adamw_update(_raw_stream(dev), C.byref(d)))

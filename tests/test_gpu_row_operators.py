@@ -352,6 +352,25 @@ def test_log_probs_masked_and_extreme_rows(cuda, dtype, v):
     assert bool(dx[~broken].isfinite().all()) and bool(dx[broken].isnan().any(1).all()) and bool(broken[5] & broken[6])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [7, 3000, 80001])
+@pytest.mark.parametrize("temperature", [1e-8, 0.01, 50.0, 100.0, 1e6])
+def test_log_probs_at_extreme_temperatures(cuda, dtype, v, temperature):
+    """-inf stays without weight and the type's lowest value keeps the one it has, whatever the temperature; values of the
+    order of the temperature, so that something is left to compare."""
+    info = torch.finfo(dtype)
+    x = rand(45, (6, v), dtype, min(2.0 * temperature, 1e4))
+    x[1, 1::2] = -INF
+    x[2] = info.min
+    x[2, ::3] = -INF
+    x[3] = -INF
+    x[3, v - 1] = info.min
+    x[4, 2:] = info.min
+    x[5, 1:] = -INF
+    target = torch.tensor([1, 0, 1, v - 1, 0, 0], device="cuda")
+    check_probs(x, target, temperature, top=min(9, v))
+
+
 def test_log_probs_many_large_values_with_one_thread(cuda):
     """Ascending, descending and strided rows, where the largest values lie close together or all belong to elements that
     one thread takes (every 4096th vector and the like): the list of candidates runs over."""

@@ -96,7 +96,7 @@ def test_log_probs_refusals():
     refused(probs(classes=0), "shape")
     refused(probs(classes=0x7fffffff), "too many classes")
     refused(probs(rows=1 << 31), "too many rows")
-    for t in (0.0, -1.0, float("nan"), float("inf")):
+    for t in (0.0, -1.0, float("nan"), float("inf"), 1e-31, 1e31):
         refused(probs(temperature=t), "temperature")
     refused(probs(top=33, top_logp=F, top_index=F + 4096), "top 33")
     refused(probs(top=5, classes=4, top_logp=F, top_index=F + 4096), "top 5")
