@@ -136,6 +136,15 @@ __device__ __forceinline__ void gstv(T* p, const V& v PXE_SITE) { if (PXE_OK_ST(
 // Around an atomic or any other access the helpers above do not cover: true when `bytes` at p may be touched.
 template <typename T>
 __device__ __forceinline__ bool gcheck(T* p PXE_SITE) { return PXE_OK_ST(T); }
+// The source of a bulk copy: true when `bytes` bytes at p may be read.
+__device__ __forceinline__ bool gcheck_range(const void* p, unsigned bytes PXE_SITE)
+{
+#ifdef PXE_BOUNDS_CHECK
+    return bounds_ok(p, bytes, 16, false, line_, file_);
+#else
+    return true;
+#endif
+}
 template <typename T>
 __device__ __forceinline__ T gatomic_add(T* p, typename same_type<T>::type v PXE_SITE) { return PXE_OK_ST(T) ? atomicAdd(p, v) : T{}; }
 

@@ -10,6 +10,7 @@
 // of the sum as it is stored, rounded to the tensor's type, because that is what the backward pass and the next layer
 // read.
 #include <algorithm>
+#include <atomic>
 
 #include "pxe_types.cuh"
 
@@ -17,7 +18,9 @@ namespace pxe {
 namespace {
 
 constexpr int kMaxChannels = 262144;
-constexpr int kMaxPartials = 592;          // rows of the weight gradient's workspace: 4 for each of 148 SMs
+// Rows of the weight gradient's workspace, one for each block: about 9.7 MB of them, but at least 148 and at most 1184 (one
+// and eight for each SM).
+inline int max_partials(int channels) { return std::max(148, std::min(1184, 2424832 / channels)); }
 
 struct NormParams {
     const void* x;
@@ -29,7 +32,7 @@ struct NormParams {
     float* scale;
     float* rstd;
     long long xs, rs, hs, ys, qs, rows;
-    int channels, weight_f32, group, groups;
+    int channels, weight_f32, group, groups, group_shift;  // group = 1 << group_shift, or 0 for the row
     float eps, inv_channels;
 };
 
@@ -46,18 +49,19 @@ struct NormBackParams {
     float inv_channels;
 };
 
-__device__ __forceinline__ float warp_sum(float v)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
-// Sum (or NaN-keeping maximum) over the blockDim.x threads of one row; `red` holds 32 floats for each row of the block.
-// Every thread of the block calls it.
+// Sum (or NaN-keeping maximum) over the blockDim.x threads of one row (a power of two up to a warp, or whole warps); `red`
+// holds a float for each warp of the row.  Every thread of the block calls it.  One barrier: calls alternate between two places for `red`, so that a place is written
+// again only after the barrier of the call in between, which all its readers have passed.
 template <bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* red)
 {
+    if (blockDim.x < 32) {
+        for (int o = blockDim.x >> 1; o > 0; o >>= 1) {
+            const float t = __shfl_xor_sync(0xffffffffu, v, o);
+            v = MAX ? max_nan(v, t) : v + t;
+        }
+        return v;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float t = __shfl_xor_sync(0xffffffffu, v, o);
@@ -65,7 +69,6 @@ __device__ __forceinline__ float row_reduce(float v, float* red)
     }
     if (blockDim.x == 32) return v;
     const int warps = blockDim.x >> 5;
-    __syncthreads();                                       // the previous use of red is over
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     float t = (threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0.0f;
@@ -99,114 +102,173 @@ __device__ __forceinline__ void load_weight(const void* weight, int weight_f32, 
     }
 }
 
-__device__ __forceinline__ float scale_of(float largest) { return max_nan(largest / kE4m3Max, kScaleMin); }
+// A thread's elements two an instruction, where there are two.
+template <int VEC>
+__device__ __forceinline__ float sum_squares(const float (&v)[VEC], float sum)
+{
+    if constexpr (VEC >= 2) {
+        unsigned long long s2 = pair(sum, 0.0f);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const unsigned long long p = pair(v[j], v[j + 1]);
+            s2 = fma2(p, p, s2);
+        }
+        float a, b;
+        unpair(s2, a, b);
+        return a + b;
+    } else {
+        return fmaf(v[0], v[0], sum);
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void scale_by(float (&v)[VEC], float rstd, const float (&w)[VEC])
+{
+    if constexpr (VEC >= 2) {
+        const unsigned long long r2 = pair(rstd, rstd);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) unpair(mul2(mul2(pair(v[j], v[j + 1]), r2), pair(w[j], w[j + 1])), v[j], v[j + 1]);
+    } else {
+        v[0] = v[0] * rstd * w[0];
+    }
+}
+__device__ __forceinline__ float warp_largest(float v)
+{
+    float r;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+template <int VEC>
+__device__ __forceinline__ float largest_of(const float (&v)[VEC])
+{
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int j = 1; j < VEC; ++j) m = max_nan(m, fabsf(v[j]));
+    return m;
+}
+
+// The first of a thread's NV vectors: a warp's vectors lie together, 32 to an access, so that one address serves them all.
+template <int VEC, int NV>
+__device__ __forceinline__ int first_column()
+{
+    return ((threadIdx.x & ~31u) * NV + (threadIdx.x & 31u)) * VEC;
+}
 
 // ---------------------------------------------------------------- forward, row in registers
-// blockDim = (tpr, rows per block).  Weights stay in registers over the block's rows while they fit.
+// blockDim = (tpr, rows per block); short rows share a warp.  While they fit, weights stay in registers over the block's rows, and the next row is
+// loaded before this one is reduced.
+constexpr int kMaxRowsPerBlock = 8;                        // of more than a warp each
+
 template <typename T, int VEC, int NV, bool Q>
-__global__ void __launch_bounds__(NV <= 2 ? 1024 : 512)
+__global__ void __launch_bounds__(512, NV * VEC <= 8 ? 2 : 1)
 rms_norm_kernel(const NormParams p)
 {
-    constexpr bool KEEP = NV * VEC <= 16;
-    __shared__ float reds[32 * 8];
+    constexpr bool KEEP = NV * VEC <= 16, AHEAD = NV * VEC <= 16;
+    constexpr int SPAN = 32 * VEC;
+    __shared__ float reds[2][kMaxRowsPerBlock][16], red_max[2][kMaxRowsPerBlock][16];
+    const int slot = blockDim.x > 32 ? threadIdx.y : 0;
     extern __shared__ unsigned int group_max[];            // Q, groups that no set of lanes of one warp covers: [rpb][groups]
-    float* red = reds + threadIdx.y * 32;
-    const int tpr = blockDim.x, rpb = blockDim.y, C = p.channels;
+    const int tpr = blockDim.x, rpb = blockDim.y, C = p.channels, col0 = first_column<VEC, NV>();
+    const T* const px = static_cast<const T*>(p.x) + col0;
+    const T* const pr = p.residual ? static_cast<const T*>(p.residual) + col0 : nullptr;
     float w[KEEP ? NV : 1][VEC];
     if constexpr (KEEP) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * tpr + threadIdx.x) * VEC;
+            const int col = col0 + i * SPAN;
             if (col < C) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[i]);
         }
     }
-    for (long long row0 = (long long)blockIdx.x * rpb; row0 < p.rows; row0 += (long long)gridDim.x * rpb) {
+    Raw<T, VEC> xr[NV], rr[NV];
+    auto load = [&](long long row) {
+        if (row >= p.rows) return;
+        const T* const x = px + row * p.xs;
+        const T* const r = pr + row * p.rs;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN;
+            if (col < C) {
+                xr[i] = gldv<Raw<T, VEC>>(x + i * SPAN);
+                if (pr) rr[i] = gldv<Raw<T, VEC>>(r + i * SPAN);
+            }
+        }
+    };
+    const long long step = (long long)gridDim.x * rpb;
+    if (AHEAD) load((long long)blockIdx.x * rpb + threadIdx.y);
+    int turn = 0;
+    for (long long row0 = (long long)blockIdx.x * rpb; row0 < p.rows; row0 += step, turn ^= 1) {
         const long long row = row0 + threadIdx.y;
         const bool active = row < p.rows;
-        const T* x = static_cast<const T*>(p.x) + row * p.xs;
-        const T* r = static_cast<const T*>(p.residual) + row * p.rs;
+        T* const h = static_cast<T*>(p.h) + row * p.hs + col0;
+        T* const y = static_cast<T*>(p.y) + row * p.ys + col0;
+        if (!AHEAD) load(row);
         float v[NV][VEC];
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * tpr + threadIdx.x) * VEC;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
-            if (active && col < C) unpack<T, VEC>(gldv<Raw<T, VEC>>(x + col), v[i]);
-        }
-        if (p.residual) {
-            T* h = static_cast<T*>(p.h) + row * p.hs;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int col = (i * tpr + threadIdx.x) * VEC;
-                if (active && col < C) {
+            const int col = col0 + i * SPAN;
+            if (active && col < C) {
+                unpack<T, VEC>(xr[i], v[i]);
+                if (pr) {
                     float a[VEC];
-                    unpack<T, VEC>(gldv<Raw<T, VEC>>(r + col), a);
+                    unpack<T, VEC>(rr[i], a);
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) a[j] += v[i][j];
                     const Raw<T, VEC> raw = pack<T, VEC>(a);
-                    gstv(h + col, raw);
+                    gstv(h + i * SPAN, raw);
                     unpack<T, VEC>(raw, v[i]);
                 }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
             }
         }
+        if (AHEAD) load(row + step);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) sum = fmaf(v[i][j], v[i][j], sum);
-        sum = row_reduce<false>(sum, red);
+        for (int i = 0; i < NV; ++i) sum = sum_squares<VEC>(v[i], sum);
+        sum = row_reduce<false>(sum, reds[turn][slot]);
         const float rstd = rsqrtf(sum * p.inv_channels + p.eps);
         if (p.rstd && active && threadIdx.x == 0) gst(p.rstd + row, rstd);
-        float largest = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * tpr + threadIdx.x) * VEC;
-            if constexpr (!KEEP) {
-                if (col < C) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
-            }
-            if (col < C) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    v[i][j] = v[i][j] * rstd * w[KEEP ? i : 0][j];
-                    if constexpr (Q) largest = max_nan(largest, fabsf(v[i][j]));
-                }
-            }
-            if constexpr (!Q) {
-                if (active && col < C) gstv(static_cast<T*>(p.y) + row * p.ys + col, pack<T, VEC>(v[i]));
+            const int col = col0 + i * SPAN;
+            if (active && col < C) {
+                if constexpr (!KEEP) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
+                scale_by<VEC>(v[i], rstd, w[KEEP ? i : 0]);
+                if constexpr (!Q) gstv(y + i * SPAN, pack<T, VEC>(v[i]));
             }
         }
         if constexpr (Q) {
-            uint8_t* q = p.q + row * p.qs;
-            auto store = [&](int i, int col, float scale) {
-                const float inv = 1.0f / scale;
+            uint8_t* const q = p.q + row * p.qs + col0;
+            auto store = [&](int i, float scale) {
+                const float inv = e4m3_inverse(scale);
                 float a[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) a[j] = v[i][j] * inv;
-                gstv(q + col, pack_e4m3<VEC>(a));
+                gstv(q + i * SPAN, pack_e4m3<VEC>(a));
             };
             if (p.group == 0) {
-                const float scale = scale_of(row_reduce<true>(largest, red));
+                float largest = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (active && col0 + i * SPAN < C) largest = max_nan(largest, largest_of<VEC>(v[i]));
+                const float scale = e4m3_scale(row_reduce<true>(largest, red_max[turn][slot]));
                 if (active && threadIdx.x == 0) gst(p.scale + row, scale);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const int col = (i * tpr + threadIdx.x) * VEC;
-                    if (active && col < C) store(i, col, scale);
+                    const int col = col0 + i * SPAN;
+                    if (active && col < C) store(i, scale);
                 }
             } else if (p.group <= 32 * VEC) {              // a group is group / VEC neighbouring lanes of one warp
                 const int lanes = p.group / VEC;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const int col = (i * tpr + threadIdx.x) * VEC;
-                    float m = 0.0f;
-                    if (col < C) {
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(v[i][j]));
-                    }
+                    const int col = col0 + i * SPAN;
+                    float m = active && col < C ? largest_of<VEC>(v[i]) : 0.0f;
                     for (int o = lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
                     if (active && col < C) {
-                        const float scale = scale_of(m);
-                        if (col % p.group == 0) gst(p.scale + row * p.groups + col / p.group, scale);
-                        store(i, col, scale);
+                        const float scale = e4m3_scale(m);
+                        if ((threadIdx.x & (lanes - 1)) == 0) gst(p.scale + row * p.groups + (col >> p.group_shift), scale);
+                        store(i, scale);
                     }
                 }
             } else {                                       // fp32 bits of |y| order as integers do, NaN above everything
@@ -216,22 +278,18 @@ rms_norm_kernel(const NormParams p)
                 __syncthreads();
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const int col = (i * tpr + threadIdx.x) * VEC;
-                    if (col < C) {
-                        float m = 0.0f;
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(v[i][j]));
-                        atomicMax(gm + col / p.group, __float_as_uint(m));
-                    }
+                    const int col = col0 + i * SPAN;
+                    const float m = warp_largest(active && col < C ? largest_of<VEC>(v[i]) : 0.0f);      // (a warp lies within a group)
+                    if (active && col < C && (threadIdx.x & 31) == 0) atomicMax(gm + (col >> p.group_shift), __float_as_uint(m));
                 }
                 __syncthreads();
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const int col = (i * tpr + threadIdx.x) * VEC;
+                    const int col = col0 + i * SPAN;
                     if (active && col < C) {
-                        const float scale = scale_of(__uint_as_float(gm[col / p.group]));
-                        if (col % p.group == 0) gst(p.scale + row * p.groups + col / p.group, scale);
-                        store(i, col, scale);
+                        const float scale = e4m3_scale(__uint_as_float(gm[col >> p.group_shift]));
+                        if ((col & (p.group - 1)) == 0) gst(p.scale + row * p.groups + (col >> p.group_shift), scale);
+                        store(i, scale);
                     }
                 }
             }
@@ -245,7 +303,7 @@ template <typename T, int VEC, bool Q>
 __global__ void __launch_bounds__(1024)
 rms_norm_long_kernel(const NormParams p)
 {
-    __shared__ float red[32];
+    __shared__ float red[32], red_max[32];
     extern __shared__ unsigned int group_max[];
     const int C = p.channels, step = blockDim.x * VEC, first = threadIdx.x * VEC;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -268,6 +326,7 @@ rms_norm_long_kernel(const NormParams p)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) sum = fmaf(v[j], v[j], sum);
         }
+        __syncthreads();
         sum = row_reduce<false>(sum, red);
         const float rstd = rsqrtf(sum * p.inv_channels + p.eps);
         if (p.rstd && threadIdx.x == 0) gst(p.rstd + row, rstd);
@@ -283,29 +342,26 @@ rms_norm_long_kernel(const NormParams p)
                 gstv(static_cast<T*>(p.y) + row * p.ys + col, pack<T, VEC>(v));
             }
         } else {
-            const int group = p.group ? p.group : C;
             __syncthreads();
             for (int g = threadIdx.x; g < p.groups; g += blockDim.x) group_max[g] = 0u;
             __syncthreads();
             float largest = 0.0f;
             for (int col = first; col < C; col += step) {
                 value(col);
-                float m = 0.0f;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(v[j]));
-                if (p.group) atomicMax(group_max + col / group, __float_as_uint(m));
+                const float m = largest_of<VEC>(v);
+                if (p.group) atomicMax(group_max + (col >> p.group_shift), __float_as_uint(m));
                 else largest = max_nan(largest, m);
             }
             if (!p.group) {
-                largest = row_reduce<true>(largest, red);
+                largest = row_reduce<true>(largest, red_max);
                 if (threadIdx.x == 0) group_max[0] = __float_as_uint(largest);
             }
             __syncthreads();
             for (int col = first; col < C; col += step) {
                 value(col);
-                const float scale = scale_of(__uint_as_float(group_max[col / group]));
-                if (col % group == 0) gst(p.scale + row * p.groups + col / group, scale);
-                const float inv = 1.0f / scale;
+                const float scale = e4m3_scale(__uint_as_float(group_max[col >> p.group_shift]));
+                if (col == (col >> p.group_shift) << p.group_shift) gst(p.scale + row * p.groups + (col >> p.group_shift), scale);
+                const float inv = e4m3_inverse(scale);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] *= inv;
                 gstv(p.q + row * p.qs + col, pack_e4m3<VEC>(v));
@@ -316,98 +372,181 @@ rms_norm_long_kernel(const NormParams p)
 }
 
 // ---------------------------------------------------------------- backward, row in registers
+// dx = rstd * u - h * (rstd * k) + dresidual with k = rstd^2 * mean(u * h), and the block's part of dweight in registers
+// over all its rows.  Up to 8 elements a thread (HOLD) u and h stay in registers as floats, the weights with them, and the
+// next row is loaded before this one is reduced; beyond that a row is held as it was loaded and converted twice.
+template <typename T, int VEC>
+__device__ __forceinline__ void times(float (&a)[VEC], const float (&w)[VEC])
+{
+    if constexpr (VEC >= 2) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) unpair(mul2(pair(a[j], a[j + 1]), pair(w[j], w[j + 1])), a[j], a[j + 1]);
+    } else {
+        a[0] *= w[0];
+    }
+}
+// acc += dy * h * rstd;  dy becomes u = dy * w;  returns dot + the sum of u * h
+template <typename T, int VEC>
+__device__ __forceinline__ float first_pass(float (&dy)[VEC], const float (&h)[VEC], const float (&w)[VEC], float rstd, float (&acc)[VEC], float dot)
+{
+    if constexpr (VEC >= 2) {
+        const unsigned long long r2 = pair(rstd, rstd);
+        unsigned long long d2 = pair(dot, 0.0f);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const unsigned long long dy2 = pair(dy[j], dy[j + 1]), h2 = pair(h[j], h[j + 1]);
+            unpair(fma2(dy2, mul2(h2, r2), pair(acc[j], acc[j + 1])), acc[j], acc[j + 1]);
+            const unsigned long long u2 = mul2(dy2, pair(w[j], w[j + 1]));
+            d2 = fma2(u2, h2, d2);
+            unpair(u2, dy[j], dy[j + 1]);
+        }
+        float d0, d1;
+        unpair(d2, d0, d1);
+        return d0 + d1;
+    } else {
+        acc[0] = fmaf(dy[0], h[0] * rstd, acc[0]);
+        dy[0] *= w[0];
+        return fmaf(dy[0], h[0], dot);
+    }
+}
+// u becomes u * rstd + (h * k + res)
+template <int VEC>
+__device__ __forceinline__ void second_pass(float (&u)[VEC], const float (&h)[VEC], const float (&res)[VEC], float rstd, float k)
+{
+    if constexpr (VEC >= 2) {
+        const unsigned long long r2 = pair(rstd, rstd), k2 = pair(k, k);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2)
+            unpair(fma2(pair(u[j], u[j + 1]), r2, fma2(pair(h[j], h[j + 1]), k2, pair(res[j], res[j + 1]))), u[j], u[j + 1]);
+    } else {
+        u[0] = fmaf(u[0], rstd, fmaf(h[0], k, res[0]));
+    }
+}
+
+// A block's part of dweight to its row of the workspace; `shared`: a row of floats where the block has several rows, which
+// are added one after the other, in a fixed order.
+template <int VEC, int NV>
+__device__ __forceinline__ void store_partial(const float (&acc)[NV][VEC], float* out, int C, int col0, float* shared)
+{
+    constexpr int SPAN = 32 * VEC;
+    auto each = [&](auto&& f) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (col0 + i * SPAN + j < C) f(col0 + i * SPAN + j, acc[i][j]);
+    };
+    if (blockDim.y == 1) {
+        if constexpr (VEC >= 4) {                          // (channels are a multiple of VEC)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; j += 4)
+                    if (col0 + i * SPAN < C) gstv(out + col0 + i * SPAN + j, make_float4(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]));
+        } else {
+            each([&](int c, float v) { gst(out + c, v); });
+        }
+        return;
+    }
+    __syncthreads();
+    for (int y = 0; y < (int)blockDim.y; ++y) {
+        if ((int)threadIdx.y == y) each([&](int c, float v) { shared[c] = y == 0 ? v : shared[c] + v; });
+        __syncthreads();
+    }
+    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < C; c += blockDim.x * blockDim.y) gst(out + c, shared[c]);
+}
+
 template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(NV * VEC <= 8 ? 1024 : NV * VEC <= 16 ? 512 : 256)
+__global__ void __launch_bounds__(512)
 rms_norm_backward_kernel(const NormBackParams p)
 {
-    __shared__ float reds[32 * 8];
+    constexpr bool HOLD = NV * VEC <= 8;
+    constexpr int SPAN = 32 * VEC;
+    __shared__ float reds[2][kMaxRowsPerBlock][16];
+    const int slot = blockDim.x > 32 ? threadIdx.y : 0;
     extern __shared__ float shared_dw[];                   // rows per block > 1: [channels]
-    float* red = reds + threadIdx.y * 32;
-    const int tpr = blockDim.x, rpb = blockDim.y, C = p.channels;
-    float acc[NV][VEC];
+    const int rpb = blockDim.y, C = p.channels, col0 = first_column<VEC, NV>();
+    const T* const pdy = static_cast<const T*>(p.dy) + col0;
+    const T* const ph = static_cast<const T*>(p.h) + col0;
+    const T* const pres = p.dres ? static_cast<const T*>(p.dres) + col0 : nullptr;
+    float acc[NV][VEC], w[HOLD ? NV : 1][VEC];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[i][j] = 0.0f;
-    for (long long row0 = (long long)blockIdx.x * rpb; row0 < p.rows; row0 += (long long)gridDim.x * rpb) {
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN;
+            if (col < C) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[i]);
+        }
+    }
+    Raw<T, VEC> dyr[NV], hr[NV], resr[NV];
+    float next_rstd = 0.0f;
+    auto load = [&](long long row) {
+        if (row >= p.rows) return;
+        next_rstd = gld(p.rstd + row);
+        const T* const dy = pdy + row * p.dys;
+        const T* const h = ph + row * p.hs;
+        const T* const res = pres + row * p.rs;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN;
+            if (col < C) {
+                dyr[i] = gldv<Raw<T, VEC>>(dy + i * SPAN);
+                hr[i] = gldv<Raw<T, VEC>>(h + i * SPAN);
+                if (pres) resr[i] = gldv<Raw<T, VEC>>(res + i * SPAN);
+            }
+        }
+    };
+    const long long step = (long long)gridDim.x * rpb;
+    if (HOLD) load((long long)blockIdx.x * rpb + threadIdx.y);
+    int turn = 0;
+    for (long long row0 = (long long)blockIdx.x * rpb; row0 < p.rows; row0 += step, turn ^= 1) {
         const long long row = row0 + threadIdx.y;
         const bool active = row < p.rows;
-        const T* dy = static_cast<const T*>(p.dy) + row * p.dys;
-        const T* h = static_cast<const T*>(p.h) + row * p.hs;
-        Raw<T, VEC> dyr[NV], hr[NV];
+        T* const dx = static_cast<T*>(p.dx) + row * p.dxs + col0;
+        if (!HOLD) load(row);
+        float u[HOLD ? NV : 1][VEC], h[HOLD ? NV : 1][VEC], res[HOLD ? NV : 1][VEC];
+        auto unpack_residual = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) res[HOLD ? i : 0][j] = 0.0f;
+            if (pres) unpack<T, VEC>(resr[i], res[HOLD ? i : 0]);
+        };
+        const float rstd = next_rstd;
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * tpr + threadIdx.x) * VEC;
-            dyr[i] = Raw<T, VEC>{};
-            hr[i] = Raw<T, VEC>{};
+            const int col = col0 + i * SPAN, k = HOLD ? i : 0;
             if (active && col < C) {
-                dyr[i] = gldv<Raw<T, VEC>>(dy + col);
-                hr[i] = gldv<Raw<T, VEC>>(h + col);
+                if constexpr (!HOLD) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
+                unpack<T, VEC>(dyr[i], u[k]);
+                unpack<T, VEC>(hr[i], h[k]);
+                if constexpr (HOLD) unpack_residual(i);
+                dot = first_pass<T, VEC>(u[k], h[k], w[k], rstd, acc[i], dot);
             }
         }
-        const float rstd = active ? gld(p.rstd + row) : 0.0f;
+        if (HOLD) load(row + step);
+        dot = row_reduce<false>(dot, reds[turn][slot]);
+        const float factor = -(dot * p.inv_channels * rstd * rstd * rstd);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * tpr + threadIdx.x) * VEC;
-            if (col < C) {
-                float a[VEC], b[VEC], w[VEC];
-                unpack<T, VEC>(dyr[i], a);
-                unpack<T, VEC>(hr[i], b);
-                load_weight<T, VEC>(p.weight, p.weight_f32, col, w);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    dot = fmaf(a[j] * w[j], b[j], dot);
-                    acc[i][j] = fmaf(a[j], b[j] * rstd, acc[i][j]);
-                }
-            }
-        }
-        dot = row_reduce<false>(dot, red);
-        const float k = dot * p.inv_channels * rstd * rstd;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = (i * tpr + threadIdx.x) * VEC;
+            const int col = col0 + i * SPAN, k = HOLD ? i : 0;
             if (active && col < C) {
-                float a[VEC], b[VEC], w[VEC];
-                unpack<T, VEC>(dyr[i], a);
-                unpack<T, VEC>(hr[i], b);
-                load_weight<T, VEC>(p.weight, p.weight_f32, col, w);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) a[j] = rstd * (a[j] * w[j] - b[j] * k);
-                if (p.dres) {
-                    unpack<T, VEC>(gldv<Raw<T, VEC>>(static_cast<const T*>(p.dres) + row * p.rs + col), b);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) a[j] += b[j];
+                if constexpr (!HOLD) {
+                    load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
+                    unpack<T, VEC>(dyr[i], u[0]);
+                    unpack<T, VEC>(hr[i], h[0]);
+                    unpack_residual(i);
+                    times<T, VEC>(u[0], w[0]);
                 }
-                gstv(static_cast<T*>(p.dx) + row * p.dxs + col, pack<T, VEC>(a));
+                second_pass<VEC>(u[k], h[k], res[k], rstd, factor);
+                gstv(dx + i * SPAN, pack<T, VEC>(u[k]));
             }
         }
     }
     if (p.partial == nullptr) return;
-    float* out = p.partial + (long long)blockIdx.x * C;
-    if (rpb == 1) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = (i * tpr + threadIdx.x) * VEC;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (col + j < C) gst(out + col + j, acc[i][j]);
-        }
-        return;
-    }
-    for (int y = 0; y < rpb; ++y) {                        // the block's rows one after the other: a fixed order
-        if ((int)threadIdx.y == y) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int col = (i * tpr + threadIdx.x) * VEC;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (col + j < C) shared_dw[col + j] = y == 0 ? acc[i][j] : shared_dw[col + j] + acc[i][j];
-            }
-        }
-        __syncthreads();
-    }
-    for (int c = threadIdx.y * tpr + threadIdx.x; c < C; c += tpr * rpb) gst(out + c, shared_dw[c]);
+    store_partial<VEC, NV>(acc, p.partial + (long long)blockIdx.x * C, C, col0, shared_dw);
 }
 
 // Any row length: the row is read twice, the block's part of the weight gradient lives in its row of the workspace.
@@ -430,6 +569,7 @@ rms_norm_backward_long_kernel(const NormBackParams p)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) dot = fmaf(a[j] * w[j], b[j], dot);
         }
+        __syncthreads();
         dot = row_reduce<false>(dot, red);
         const float k = dot * p.inv_channels * rstd * rstd;
         for (int col = first; col < C; col += step) {
@@ -455,21 +595,271 @@ rms_norm_backward_long_kernel(const NormBackParams p)
     }
 }
 
-// dweight[c] = the sum of column c over the workspace's rows: 32 columns by 16 row groups to a block, each group's rows
-// and then the groups in order.
+// ---------------------------------------------------------------- many rows of whole vectors: a ring of rows in shared memory
+// The forms above wait for one row while they work on another; that leaves too few bytes on their way (a row's chain of
+// load, barrier, reduction and store takes about 1.5 us, whatever it moves).  Here one thread keeps `stages` rows of
+// every input coming in with bulk copies.  A row's barrier in its reduction says that all threads are done with the row
+// before, whose place is then refilled.  Waits are bounded: a copy that never completes leaves NaN behind, not a hang.
+constexpr int kMaxStages = 8;
+constexpr int kWaitLimit = 1 << 20;
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+struct Ring {
+    unsigned char* data;                                   // [stages][stage_bytes]
+    unsigned long long* full;                              // [stages]
+    int stages, stage_bytes;
+    __device__ __forceinline__ void init() const
+    {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < stages; ++i) asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(shared_address(full + i)) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncthreads();
+    }
+    // One thread: a row of `bytes` bytes of each of n tensors into a stage.
+    template <int N>
+    __device__ __forceinline__ void fill(int stage, const void* const (&src)[N], int n, int bytes) const
+    {
+        const uint32_t bar = shared_address(full + stage);
+        int expected = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < n && gcheck_range(src[k], bytes)) expected += bytes;
+        asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(expected) : "memory");
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < n && gcheck_range(src[k], bytes))
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                 shared_address(data + stage * stage_bytes + k * bytes)),
+                             "l"(src[k]), "r"(bytes), "r"(bar)
+                             : "memory");
+    }
+    __device__ __forceinline__ bool wait(int stage, int parity) const
+    {
+        const uint32_t bar = shared_address(full + stage);
+        for (int i = 0; i < kWaitLimit; ++i) {
+            uint32_t done;
+            asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+            if (done) return true;
+        }
+        return false;
+    }
+    template <typename V>
+    static __device__ __forceinline__ V read(const unsigned char* p) { return *reinterpret_cast<const V*>(p); }
+};
+
+extern __shared__ __align__(128) unsigned char ring_shared[];
+
+template <typename T, int NV, bool Q>
 __global__ void __launch_bounds__(512)
+rms_norm_ring_kernel(const NormParams p, int stages)
+{
+    constexpr int VEC = 16 / sizeof(T), SPAN = 32 * VEC;
+    constexpr bool KEEP = NV * VEC <= 16;
+    __shared__ float reds[2][16], red_max[2][16];
+    __shared__ unsigned long long full[kMaxStages];
+    const int C = p.channels, col0 = first_column<VEC, NV>(), bytes = C * (int)sizeof(T), inputs = p.residual ? 2 : 1;
+    const Ring ring{ring_shared, full, stages, bytes * inputs};
+    ring.init();
+    auto fill = [&](int stage, long long row) {
+        const void* const src[2] = {static_cast<const T*>(p.x) + row * p.xs, static_cast<const T*>(p.residual) + row * p.rs};
+        ring.fill<2>(stage, src, inputs, bytes);
+    };
+    const long long step = gridDim.x;
+    if (threadIdx.x == 0)
+        for (int i = 0; i < stages; ++i)
+            if (blockIdx.x + i * step < p.rows) fill(i, blockIdx.x + i * step);
+    float w[KEEP ? NV : 1][VEC];
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN;
+            if (col < C) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[i]);
+        }
+    }
+    int stage = 0, parity = 0, turn = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += step, turn ^= 1) {
+        const bool arrived = ring.wait(stage, parity);
+        const unsigned char* const at = ring.data + stage * ring.stage_bytes + col0 * (int)sizeof(T);
+        const unsigned char* const at2 = at + bytes;
+        T* const h = static_cast<T*>(p.h) + row * p.hs + col0;
+        T* const y = static_cast<T*>(p.y) + row * p.ys + col0;
+        uint8_t* const q = p.q + row * p.qs + col0;
+        float v[NV][VEC];
+        float sum = arrived ? 0.0f : __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN;
+            if (col < C) {
+                unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + i * SPAN * (int)sizeof(T)), v[i]);
+                if (p.residual) {
+                    float a[VEC];
+                    unpack<T, VEC>(ring.read<Raw<T, VEC>>(at2 + i * SPAN * (int)sizeof(T)), a);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) a[j] += v[i][j];
+                    const Raw<T, VEC> raw = pack<T, VEC>(a);
+                    gstv(h + i * SPAN, raw);
+                    unpack<T, VEC>(raw, v[i]);
+                }
+                sum = sum_squares<VEC>(v[i], sum);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
+            }
+        }
+        sum = row_reduce<false>(sum, reds[turn]);
+        const int before = stage == 0 ? stages - 1 : stage - 1;
+        if (threadIdx.x == 0 && row != blockIdx.x && row + (stages - 1) * step < p.rows) fill(before, row + (stages - 1) * step);
+        const float rstd = rsqrtf(sum * p.inv_channels + p.eps);
+        if (p.rstd && threadIdx.x == 0) gst(p.rstd + row, rstd);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN;
+            if (col < C) {
+                if constexpr (!KEEP) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
+                scale_by<VEC>(v[i], rstd, w[KEEP ? i : 0]);
+                if constexpr (!Q) gstv(y + i * SPAN, pack<T, VEC>(v[i]));
+            }
+        }
+        if constexpr (Q) {
+            auto store = [&](int i, float scale) {
+                const float inv = e4m3_inverse(scale);
+                float a[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) a[j] = v[i][j] * inv;
+                gstv(q + i * SPAN, pack_e4m3<VEC>(a));
+            };
+            if (p.group == 0) {
+                float largest = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (col0 + i * SPAN < C) largest = max_nan(largest, largest_of<VEC>(v[i]));
+                const float scale = e4m3_scale(row_reduce<true>(largest, red_max[turn]));
+                if (threadIdx.x == 0) gst(p.scale + row, scale);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int col = col0 + i * SPAN;
+                    if (col < C) store(i, scale);
+                }
+            } else {                                       // a group is group / VEC neighbouring lanes of one warp
+                const int lanes = p.group / VEC;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int col = col0 + i * SPAN;
+                    float m = col < C ? largest_of<VEC>(v[i]) : 0.0f;
+                    for (int o = lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    if (col < C) {
+                        const float scale = e4m3_scale(m);
+                        if ((threadIdx.x & (lanes - 1)) == 0) gst(p.scale + row * p.groups + (col >> p.group_shift), scale);
+                        store(i, scale);
+                    }
+                }
+            }
+        }
+        if (++stage == stages) { stage = 0; parity ^= 1; }
+    }
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(512)
+rms_norm_backward_ring_kernel(const NormBackParams p, int stages)
+{
+    constexpr int VEC = 16 / sizeof(T), SPAN = 32 * VEC;
+    constexpr bool HOLD = NV * VEC <= 8;
+    __shared__ float reds[2][16];
+    __shared__ unsigned long long full[kMaxStages];
+    const int C = p.channels, col0 = first_column<VEC, NV>(), bytes = C * (int)sizeof(T), inputs = p.dres ? 3 : 2;
+    const Ring ring{ring_shared, full, stages, bytes * inputs};
+    ring.init();
+    auto fill = [&](int stage, long long row) {
+        const void* const src[3] = {static_cast<const T*>(p.dy) + row * p.dys, static_cast<const T*>(p.h) + row * p.hs, static_cast<const T*>(p.dres) + row * p.rs};
+        ring.fill<3>(stage, src, inputs, bytes);
+    };
+    const long long step = gridDim.x;
+    if (threadIdx.x == 0)
+        for (int i = 0; i < stages; ++i)
+            if (blockIdx.x + i * step < p.rows) fill(i, blockIdx.x + i * step);
+    float acc[NV][VEC], w[HOLD ? NV : 1][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[i][j] = 0.0f;
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN;
+            if (col < C) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[i]);
+        }
+    }
+    float next_rstd = gld(p.rstd + blockIdx.x);            // (there are at least two rows for each block)
+    int stage = 0, parity = 0, turn = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += step, turn ^= 1) {
+        const float rstd = next_rstd;
+        if (row + step < p.rows) next_rstd = gld(p.rstd + row + step);
+        const bool arrived = ring.wait(stage, parity);
+        const unsigned char* const at = ring.data + stage * ring.stage_bytes + col0 * (int)sizeof(T);
+        const unsigned char* const at2 = at + bytes;
+        const unsigned char* const at3 = at2 + bytes;
+        T* const dx = static_cast<T*>(p.dx) + row * p.dxs + col0;
+        float u[HOLD ? NV : 1][VEC], h[HOLD ? NV : 1][VEC];
+        float dot = arrived ? 0.0f : __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN, k = HOLD ? i : 0;
+            if (col < C) {
+                if constexpr (!HOLD) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
+                unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + i * SPAN * (int)sizeof(T)), u[k]);
+                unpack<T, VEC>(ring.read<Raw<T, VEC>>(at2 + i * SPAN * (int)sizeof(T)), h[k]);
+                dot = first_pass<T, VEC>(u[k], h[k], w[k], rstd, acc[i], dot);
+            }
+        }
+        dot = row_reduce<false>(dot, reds[turn]);
+        const int before = stage == 0 ? stages - 1 : stage - 1;
+        if (threadIdx.x == 0 && row != blockIdx.x && row + (stages - 1) * step < p.rows) fill(before, row + (stages - 1) * step);
+        const float factor = -(dot * p.inv_channels * rstd * rstd * rstd);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = col0 + i * SPAN, k = HOLD ? i : 0;
+            if (col < C) {
+                if constexpr (!HOLD) {
+                    load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
+                    unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + i * SPAN * (int)sizeof(T)), u[0]);
+                    unpack<T, VEC>(ring.read<Raw<T, VEC>>(at2 + i * SPAN * (int)sizeof(T)), h[0]);
+                    times<T, VEC>(u[0], w[0]);
+                }
+                float res[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) res[j] = 0.0f;
+                if (p.dres) unpack<T, VEC>(ring.read<Raw<T, VEC>>(at3 + i * SPAN * (int)sizeof(T)), res);
+                second_pass<VEC>(u[k], h[k], res, rstd, factor);
+                gstv(dx + i * SPAN, pack<T, VEC>(u[k]));
+            }
+        }
+        if (++stage == stages) { stage = 0; parity ^= 1; }
+    }
+    if (p.partial == nullptr) return;
+    store_partial<VEC, NV>(acc, p.partial + (long long)blockIdx.x * C, C, col0, nullptr);
+}
+
+// dweight[c] = the sum of column c over the workspace's rows: 16 columns by 64 row groups to a block, each group's rows and
+// then the groups in order.  Launched while the kernel that fills the workspace still runs; it waits for that one's end.
+__global__ void __launch_bounds__(1024)
 rms_norm_dweight_kernel(const float* partial, int parts, int channels, float* dweight, int accumulate)
 {
-    __shared__ float part[16][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;
+    __shared__ float part[64][17];
+    const int c = blockIdx.x * 16 + threadIdx.x;
     float sum = 0.0f;
-    if (c < channels)
-        for (int r = threadIdx.y; r < parts; r += 16) sum += gld(partial + (long long)r * channels + c);
+    cudaGridDependencySynchronize();
+    if (c < channels) {
+#pragma unroll 10
+        for (int r = threadIdx.y; r < parts; r += 64) sum += gld(partial + (long long)r * channels + c);
+    }
     part[threadIdx.y][threadIdx.x] = sum;
     __syncthreads();
     if (threadIdx.y == 0 && c < channels) {
 #pragma unroll
-        for (int y = 1; y < 16; ++y) sum += part[y][threadIdx.x];
+        for (int y = 1; y < 64; ++y) sum += part[y][threadIdx.x];
         gst(dweight + c, accumulate ? gld(dweight + c) + sum : sum);
     }
 }
@@ -489,23 +879,99 @@ struct Layout {
     int tpr, rpb;
 };
 
-// Threads and registers for rows of `channels`: up to 256 threads take one vector each and longer rows two, then four and
-// eight (more bytes in flight for a thread, fewer warps to reduce over); with `few` rows the row is spread over as many
-// threads as there are vectors, up to a block's limit.
-Layout layout_for(int vec, int channels, bool few, int max_nv, int max_threads_nv1)
+// Threads and registers for rows of `channels`.  What a row costs whatever its length (two trees of shuffles, a barrier)
+// wants few threads with much each: rows that a warp holds with up to eight accesses or 32 bytes of a tensor a lane (forward,
+// one whole vector) take a warp (or the power of two of its lanes that is enough), longer ones as many threads with as much, up to 512, then with
+// 64 bytes.  With `few` rows (less than one for each SM), where nothing but a row's own time counts, one access up to 512
+// threads; backward, where a thread holds three tensors and a sum for each element, up to 8 elements first.
+Layout layout_for(int vec, int size, int channels, bool few, bool backward)
 {
     Layout l{vec, 1, 32, 1};
-    const int vecs = (channels + vec - 1) / vec;
-    int nv = 1;
-    if (few) while (nv <= max_nv && (long long)nv * max_threads_nv1 < vecs) nv *= 2;
-    else while (nv <= max_nv && (long long)nv * 256 < vecs && nv < 4) nv *= 2;
-    auto limit = [&](int n) { return n <= 2 ? max_threads_nv1 : 512; };
-    while (nv <= max_nv && (long long)nv * limit(nv) < vecs) nv *= 2;
-    if (nv > max_nv) { l.nv = 0; l.tpr = 1024; return l; }
-    l.nv = nv;
-    l.tpr = ((vecs + nv - 1) / nv + 31) / 32 * 32;
-    l.rpb = l.tpr <= 128 ? std::min(8, 256 / l.tpr) : 1;
+    const int vecs = (channels + vec - 1) / vec, most = vec * size == 16 && !backward ? 1 : std::min(8, 32 / (vec * size));
+    if (vecs <= 32) {
+        l.tpr = 1;
+        while (l.tpr < vecs) l.tpr *= 2;
+        l.rpb = 256 / l.tpr;
+        return l;
+    }
+    if (!few) {
+        while (l.nv < most && l.nv * 32 < vecs) l.nv *= 2;
+        if (l.nv * 32 >= vecs) {
+            l.rpb = 8;
+            return l;
+        }
+        if (backward) l.nv = std::min(most, std::max(1, 8 / vec));
+    }
+    while (l.nv * 512 < vecs) l.nv *= 2;
+    if (l.nv > 8 || l.nv * vec * size > 64) {
+        l.nv = 0;
+        l.tpr = 1024;
+        return l;
+    }
+    l.tpr = ((vecs + l.nv - 1) / l.nv + 31) / 32 * 32;
+    l.rpb = l.tpr <= 128 ? std::min(kMaxRowsPerBlock, 256 / l.tpr) : 1;
     return l;
+}
+
+// The ring form takes rows of 2 to 32 KB in whole vectors, when there are enough of them to fill the card: as many threads
+// as the row needs with one vector each, then two, up to 512 threads with four; 1024 threads to an SM (512 where a thread
+// holds four), and the stages that seven eighths of the shared memory hold.
+struct RingLayout {
+    int nv, tpr, blocks_per_sm, stages;
+    size_t shared;
+};
+bool ring_layout(int size, int channels, int inputs, long long rows, const DeviceInfo& di, RingLayout* l)
+{
+    const int bytes = channels * size, vecs = bytes / 16;
+    if (bytes < 2048 || bytes > 32768) return false;
+    l->nv = vecs <= 256 ? 1 : vecs <= 1024 ? 2 : 4;
+    l->tpr = ((vecs + l->nv - 1) / l->nv + 31) / 32 * 32;
+    l->blocks_per_sm = std::max(1, (l->nv == 4 ? 512 : 1024) / l->tpr);
+    if (rows < 2LL * di.sm_count * l->blocks_per_sm) return false;
+    l->stages = (int)std::min<long long>(kMaxStages, (long long)di.max_smem_optin * 7 / 8 / l->blocks_per_sm / (bytes * inputs));
+    l->shared = (size_t)l->stages * bytes * inputs;
+    return l->stages >= 2;
+}
+
+// Allows a kernel its dynamic shared memory, once for each device.
+template <typename K>
+int allow_shared(K kernel, int device, int bytes, std::atomic<unsigned long long>& done)
+{
+    if (done.load(std::memory_order_relaxed) >> device & 1) return PXE_OK;
+    PXE_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(1ull << device, std::memory_order_relaxed);
+    return PXE_OK;
+}
+
+template <typename T, int NV, bool Q>
+int launch_norm_ring(cudaStream_t s, const NormParams& p, const RingLayout& l, const DeviceInfo& di, int device)
+{
+    static std::atomic<unsigned long long> done{0};
+    { const int rc = allow_shared(rms_norm_ring_kernel<T, NV, Q>, device, di.max_smem_optin - 4096, done); if (rc != PXE_OK) return rc; }
+    rms_norm_ring_kernel<T, NV, Q><<<(unsigned)(di.sm_count * l.blocks_per_sm), l.tpr, l.shared, s>>>(p, l.stages);
+    PXE_LAUNCH_OK("rms_norm_ring_kernel");
+    return PXE_OK;
+}
+template <typename T, bool Q>
+int launch_norm_ring(cudaStream_t s, const NormParams& p, const RingLayout& l, const DeviceInfo& di, int device)
+{
+    return l.nv == 1 ? launch_norm_ring<T, 1, Q>(s, p, l, di, device) : l.nv == 2 ? launch_norm_ring<T, 2, Q>(s, p, l, di, device)
+                                                                                   : launch_norm_ring<T, 4, Q>(s, p, l, di, device);
+}
+template <typename T, int NV>
+int launch_backward_ring(cudaStream_t s, const NormBackParams& p, const RingLayout& l, const DeviceInfo& di, int device)
+{
+    static std::atomic<unsigned long long> done{0};
+    { const int rc = allow_shared(rms_norm_backward_ring_kernel<T, NV>, device, di.max_smem_optin - 4096, done); if (rc != PXE_OK) return rc; }
+    rms_norm_backward_ring_kernel<T, NV><<<(unsigned)(di.sm_count * l.blocks_per_sm), l.tpr, l.shared, s>>>(p, l.stages);
+    PXE_LAUNCH_OK("rms_norm_backward_ring_kernel");
+    return PXE_OK;
+}
+template <typename T>
+int launch_backward_ring(cudaStream_t s, const NormBackParams& p, const RingLayout& l, const DeviceInfo& di, int device)
+{
+    return l.nv == 1 ? launch_backward_ring<T, 1>(s, p, l, di, device) : l.nv == 2 ? launch_backward_ring<T, 2>(s, p, l, di, device)
+                                                                                    : launch_backward_ring<T, 4>(s, p, l, di, device);
 }
 
 template <typename T, int VEC, bool Q>
@@ -527,7 +993,9 @@ int launch_norm(cudaStream_t s, const NormParams& p, const Layout& l, const Devi
     case 1: rms_norm_kernel<T, VEC, 1, Q><<<grid, block, smem, s>>>(p); break;
     case 2: rms_norm_kernel<T, VEC, 2, Q><<<grid, block, smem, s>>>(p); break;
     case 4: rms_norm_kernel<T, VEC, 4, Q><<<grid, block, smem, s>>>(p); break;
-    default: rms_norm_kernel<T, VEC, 8, Q><<<grid, block, smem, s>>>(p); break;
+    default:
+        if constexpr (VEC <= 2) rms_norm_kernel<T, VEC, 8, Q><<<grid, block, smem, s>>>(p);
+        break;
     }
     PXE_LAUNCH_OK("rms_norm_kernel");
     return PXE_OK;
@@ -546,7 +1014,10 @@ int launch_backward(cudaStream_t s, const NormBackParams& p, const Layout& l, un
     switch (l.nv) {
     case 1: rms_norm_backward_kernel<T, VEC, 1><<<grid, block, smem, s>>>(p); break;
     case 2: rms_norm_backward_kernel<T, VEC, 2><<<grid, block, smem, s>>>(p); break;
-    default: rms_norm_backward_kernel<T, VEC, 4><<<grid, block, smem, s>>>(p); break;
+    case 4: rms_norm_backward_kernel<T, VEC, 4><<<grid, block, smem, s>>>(p); break;
+    default:
+        if constexpr (VEC <= 2) rms_norm_backward_kernel<T, VEC, 8><<<grid, block, smem, s>>>(p);
+        break;
     }
     PXE_LAUNCH_OK("rms_norm_backward_kernel");
     return PXE_OK;
@@ -585,8 +1056,9 @@ extern "C" int pxe_rms_norm(pxe_stream_t stream, const pxe_rms_norm_desc* dp)
     p.x = d.x; p.residual = d.residual; p.weight = d.weight; p.h = d.h; p.y = d.y; p.q = static_cast<uint8_t*>(d.q);
     p.scale = d.scale; p.rstd = d.rstd;
     p.rows = d.rows; p.channels = C; p.weight_f32 = d.weight_type == PXE_F32;
-    p.group = d.q ? d.group : 0;
+    p.group = d.q && d.group < C ? d.group : 0;            // one group is the row
     p.groups = p.group ? (C + p.group - 1) / p.group : 1;
+    p.group_shift = p.group == 32 ? 5 : p.group == 64 ? 6 : p.group == 128 ? 7 : 30;
     p.eps = d.eps; p.inv_channels = 1.0f / (float)C;
     const struct { const char* name; const void* ptr; long long given; long long* stride; int bytes; } tensors[] = {
         {"x", d.x, d.x_row_stride, &p.xs, size}, {"residual", d.residual, d.residual_row_stride, &p.rs, size},
@@ -618,8 +1090,16 @@ extern "C" int pxe_rms_norm(pxe_stream_t stream, const pxe_rms_norm_desc* dp)
                     !(d.q && rows_conflict(span[i], scales)), "rms_norm: rstd or scale overlaps %s", tensors[i].name);
     DeviceInfo di;
     { const int rc = device_info(&di); if (rc != PXE_OK) return rc; }
-    const Layout l = layout_for(vec, C, d.rows < di.sm_count, 8, 1024);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    RingLayout rl;
+    if (vec * size == 16 && ring_layout(size, C, d.residual ? 2 : 1, d.rows, di, &rl)) {
+        int device = 0;
+        PXE_CUDA_OK(cudaGetDevice(&device));
+        if (d.type == PXE_F32) return d.q ? launch_norm_ring<float, true>(s, p, rl, di, device) : launch_norm_ring<float, false>(s, p, rl, di, device);
+        if (d.type == PXE_BF16) return d.q ? launch_norm_ring<bf16, true>(s, p, rl, di, device) : launch_norm_ring<bf16, false>(s, p, rl, di, device);
+        return d.q ? launch_norm_ring<f16, true>(s, p, rl, di, device) : launch_norm_ring<f16, false>(s, p, rl, di, device);
+    }
+    const Layout l = layout_for(vec, size, C, d.rows < di.sm_count, false);
 #define PXE_NORM_VEC(T, V) return d.q ? launch_norm<T, V, true>(s, p, l, di) : launch_norm<T, V, false>(s, p, l, di)
     if (d.type == PXE_F32) { if (vec == 4) PXE_NORM_VEC(float, 4); PXE_NORM_VEC(float, 1); }
     if (d.type == PXE_BF16) { if (vec == 8) PXE_NORM_VEC(bf16, 8); if (vec == 2) PXE_NORM_VEC(bf16, 2); PXE_NORM_VEC(bf16, 1); }
@@ -632,7 +1112,7 @@ extern "C" int pxe_rms_norm(pxe_stream_t stream, const pxe_rms_norm_desc* dp)
 extern "C" size_t pxe_rms_norm_backward_workspace_bytes(long long rows, int channels)
 {
     if (rows <= 0 || channels <= 0) return 0;
-    return (size_t)std::min<long long>(rows, kMaxPartials) * channels * 4;
+    return (size_t)std::min<long long>(rows, max_partials(channels)) * channels * 4;
 }
 
 extern "C" int pxe_rms_norm_backward(pxe_stream_t stream, const pxe_rms_norm_backward_desc* dp)
@@ -687,27 +1167,33 @@ extern "C" int pxe_rms_norm_backward(pxe_stream_t stream, const pxe_rms_norm_bac
     if (d.weight && widest(d.weight, 0) < std::min(16, vec * wsize)) vec = 1;
     DeviceInfo di;
     { const int rc = device_info(&di); if (rc != PXE_OK) return rc; }
-    // a thread holds 8, 16 or 32 elements of the weight gradient: up to 1024, 512, 256 threads
-    Layout l{vec, 1, 32, 1};
-    const int vecs = (C + vec - 1) / vec;
-    int nv = 1;
-    while (nv < 4 && nv * 256 < vecs) nv *= 2;
-    while (nv > 1 && nv * (nv * vec <= 8 ? 1024 : nv * vec <= 16 ? 512 : 256) < vecs) nv /= 2;
-    if (nv * (nv * vec <= 8 ? 1024 : nv * vec <= 16 ? 512 : 256) < vecs) {
-        l.nv = 0; l.tpr = 1024;
-    } else {
-        l.nv = nv;
-        l.tpr = ((vecs + nv - 1) / nv + 31) / 32 * 32;
-        l.rpb = l.tpr <= 128 ? std::min(8, 256 / l.tpr) : 1;
-    }
-    const long long blocks = (d.rows + l.rpb - 1) / l.rpb;
-    const unsigned grid = (unsigned)std::min<long long>(std::min<long long>(blocks, kMaxPartials), (long long)di.sm_count * std::max(1, 1024 / (l.tpr * l.rpb)));
     int rc;
-    if (d.type == PXE_F32) rc = vec == 4 ? launch_backward<float, 4>(s, p, l, grid) : launch_backward<float, 1>(s, p, l, grid);
-    else if (d.type == PXE_BF16) rc = vec == 8 ? launch_backward<bf16, 8>(s, p, l, grid) : vec == 2 ? launch_backward<bf16, 2>(s, p, l, grid) : launch_backward<bf16, 1>(s, p, l, grid);
-    else rc = vec == 8 ? launch_backward<f16, 8>(s, p, l, grid) : vec == 2 ? launch_backward<f16, 2>(s, p, l, grid) : launch_backward<f16, 1>(s, p, l, grid);
+    unsigned grid;
+    RingLayout rl;
+    if (vec * size == 16 && ring_layout(size, C, d.dresidual ? 3 : 2, d.rows, di, &rl) && di.sm_count * rl.blocks_per_sm <= max_partials(C)) {
+        int device = 0;
+        PXE_CUDA_OK(cudaGetDevice(&device));
+        grid = (unsigned)(di.sm_count * rl.blocks_per_sm);
+        rc = d.type == PXE_F32 ? launch_backward_ring<float>(s, p, rl, di, device) : d.type == PXE_BF16 ? launch_backward_ring<bf16>(s, p, rl, di, device)
+                                                                                                        : launch_backward_ring<f16>(s, p, rl, di, device);
+    } else {
+        const Layout l = layout_for(vec, size, C, false, true);
+        const long long blocks = (d.rows + l.rpb - 1) / l.rpb;
+        grid = (unsigned)std::min<long long>(std::min<long long>(blocks, max_partials(C)), (long long)di.sm_count * std::max(1, 1024 / (l.tpr * l.rpb)));
+        if (d.type == PXE_F32) rc = vec == 4 ? launch_backward<float, 4>(s, p, l, grid) : launch_backward<float, 1>(s, p, l, grid);
+        else if (d.type == PXE_BF16) rc = vec == 8 ? launch_backward<bf16, 8>(s, p, l, grid) : vec == 2 ? launch_backward<bf16, 2>(s, p, l, grid) : launch_backward<bf16, 1>(s, p, l, grid);
+        else rc = vec == 8 ? launch_backward<f16, 8>(s, p, l, grid) : vec == 2 ? launch_backward<f16, 2>(s, p, l, grid) : launch_backward<f16, 1>(s, p, l, grid);
+    }
     if (rc != PXE_OK || !d.dweight) return rc;
-    rms_norm_dweight_kernel<<<(C + 31) / 32, dim3(32, 16), 0, s>>>(p.partial, (int)grid, C, d.dweight, d.accumulate);
-    PXE_LAUNCH_OK("rms_norm_dweight_kernel");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((C + 15) / 16);
+    cfg.blockDim = dim3(16, 64);
+    cfg.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    PXE_CUDA_OK(cudaLaunchKernelEx(&cfg, rms_norm_dweight_kernel, (const float*)p.partial, (int)grid, C, d.dweight, d.accumulate));
     return PXE_OK;
 }

@@ -114,6 +114,52 @@ def test_rms_norm_e4m3_equals_64_bits(cuda, dtype, shape, group, pad, shift):
     within(got, y64, y64.abs() * (2.0 ** -4 * 1.001 + 2 * rel) + each * 2.0 ** -10 * 1.001)
 
 
+MANY = [(torch.bfloat16, 5000, 512), (torch.bfloat16, 2500, 2048), (torch.float16, 2600, 4096), (torch.bfloat16, 1300, 5120), (torch.float32, 1500, 4096),
+        (torch.bfloat16, 700, 16384), (torch.float32, 10000, 256), (torch.float16, 1203, 8192), (torch.bfloat16, 3001, 1032)]
+
+
+@pytest.mark.parametrize("dtype,n,c", MANY)
+@pytest.mark.parametrize("pad", [0, 64])
+def test_norms_of_many_rows_equal_64_bits(cuda, dtype, n, c, pad):
+    """Enough rows for every block to take several, in whole vectors: forward in both outputs and backward, with and
+    without the residual, in place as well."""
+    w = rand(46, (c,))
+    rel = (norm_chain(c) / 2 + 9) * U
+    for with_res in (True, False):
+        x = rand(47, (n, c), dtype, 1.0, pad)
+        res = rand(48, (n, c), dtype, 1.0, pad) if with_res else None
+        y, h, rstd = ops.rms_norm(x, w, residual=res, eps=1e-6)
+        h64, r64, y64 = norm64(x, w, res, 1e-6)
+        assert torch.equal(h, h64)
+        within(rstd, r64, r64 * rel)
+        within(y, y64, y64.abs() * rel + half_step(dtype, y64 * (1 + 1e-3)))
+        for group in (0, 128):
+            q, scale, h2, _ = ops.rms_norm_e4m3(x, w, residual=res, eps=1e-6, group=group)
+            g = group or c
+            groups = -(-c // g)
+            wide = torch.zeros(n, groups * g, dtype=torch.float64, device="cuda")
+            wide[:, :c] = y64
+            s64 = (wide.view(n, groups, g).abs().amax(-1) / 448).clamp(min=2.0 ** -126)
+            within(scale, s64, s64 * (rel + 2 * U))
+            each = s64.repeat_interleave(g, 1)[:, :c]
+            within(q.double() * scale.double().repeat_interleave(g, 1)[:, :c], y64, y64.abs() * (2.0 ** -4 * 1.001 + 2 * rel) + each * 2.0 ** -10 * 1.001)
+            assert torch.equal(h2, h)
+        dy, dres = rand(49, (n, c), dtype, 1.0, pad), rand(50, (n, c), dtype, 1.0, pad) if with_res else None
+        dx, dw = ops.rms_norm_backward(dy, h, w, rstd, dresidual=dres)
+        hd, u, r = h.double(), dy.double() * w.double(), rstd.double()[:, None]
+        mean, terms = (u * hd).mean(1, keepdim=True), dy.double() * hd * r
+        dx64 = r * (u - hd * r * r * mean) + (dres.double() if with_res else 0.0)
+        spread = r * (u.abs() + hd.abs() * r * r * (u * hd).abs().mean(1, keepdim=True) * (norm_chain(c) + 8)) * 6 * U
+        within(dx, dx64, spread + 2 * U * dx64.abs() + half_step(dtype, dx64.abs() + spread))
+        within(dw, terms.sum(0), (n / 148 + 8 + 40 + 32 + 3) * U * terms.abs().sum(0))
+        if with_res:
+            xin, rin = x.clone(), res.clone()
+            y2, h2, _ = ops.rms_norm(xin, w, residual=rin, eps=1e-6, out=xin, residual_out=rin)
+            assert torch.equal(y2, y) and torch.equal(h2, h)
+            again, dw2 = ops.rms_norm_backward(dy, h, w, rstd, dresidual=dres, dx=dres)
+            assert torch.equal(again, dx) and torch.equal(dw2, dw)
+
+
 def test_rms_norm_special_rows(cuda):
     """Zeros, NaN, infinities and values whose squares overflow stay in their row and mean what IEEE arithmetic says."""
     for dtype in TYPES:
