@@ -5,15 +5,17 @@
 // Bound by memory: every element's parameter, gradient and moments are read once and all but the gradient written once
 // (28 bytes in fp32, 16 with states in 8 bits).  The tensors' addresses travel as the kernel's parameters (72 bytes
 // each, 400 to a launch), so a call needs no table in device memory, no copy and no workspace, and a captured call keeps
-// its own.  A block of 256 threads takes chunks of 4096 elements; it finds a chunk's tensor by bisection over the first
-// chunk of each.  A warp takes 256 elements at a time, eight to a lane: that is also the block of elements that shares a
-// scale in 8 bits, so the new scale is one reduction over the warp and nothing is read twice.
+// its own.  A block of 256 threads takes 2048 elements of one tensor, which it finds by bisection over the first block of
+// each.  A warp takes 256 elements, eight to a lane: that is also the block of elements that shares a scale in 8 bits, so
+// the new scale is one reduction over the warp and nothing is read twice.  There is no loop: what hides a warp's loads is
+// the other warps of the SM and the blocks that follow.
 //
 // In 8 bits m is held as an e4m3 code times its block's scale, and v as the code of its root: the update needs the root,
 // and its codes then reach 2^-18 of the block's largest value (2^-36 in v).  A v above zero keeps the smallest code
 // instead of rounding to zero, which would leave a later step to divide by eps alone.
 #include <algorithm>
 #include <exception>
+#include <type_traits>
 #include <vector>
 
 #include "pxe_types.cuh"
@@ -23,7 +25,7 @@ namespace {
 
 constexpr int kUnit = PXE_ADAMW_BLOCK;                     // elements a warp takes at a time
 constexpr int kThreads = 256;
-constexpr int kChunk = 4096;
+constexpr int kElements = kThreads / 32 * kUnit;           // of a block
 
 struct Entry {
     void* p;
@@ -34,7 +36,7 @@ struct Entry {
     float* vs;
     float* w;
     long long n;
-    int first_chunk;
+    int first_block;
     int vector;                                            // every pointer allows whole accesses
 };
 
@@ -45,130 +47,179 @@ struct AdamwParams {
     const long long* t_device;
     const float* grad_scale_device;
     const float* skip_device;
-    int count, chunks;
+    int count, blocks;
     Entry e[MAX];
 };
 
+// The hardware's root and reciprocal (one unit in the last place; subnormal arguments kept, unlike the .ftz forms): an
+// update is off by a few units of 2^-23 of itself, far below the parameter's own rounding.
+__device__ __forceinline__ float root(float x)
+{
+    float y;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float reciprocal(float x)
+{
+    float y;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 struct Step {
-    float rate, b1, b2, omb1, omb2, eps, decay, grad_scale, inv_c1, inv_c2;
-    // the new moments and parameter of one element
-    __device__ __forceinline__ void operator()(float& p, float g, float& m, float& v) const
+    float b1, b2, omb1, omb2, eps, keep, grad_scale, step, inv_root_c2;           // keep = 1 - rate * decay, step = rate / c1
+    // the new moments and parameter of one element, and the second moment's root
+    __device__ __forceinline__ float operator()(float& p, float g, float& m, float& v) const
     {
         g *= grad_scale;
         m = fmaf(omb1, g, b1 * m);
         v = fmaf(omb2 * g, g, b2 * v);
-        p -= rate * (m * inv_c1 / (sqrtf(v * inv_c2) + eps) + decay * p);
+        const float r = root(v);
+        p = fmaf(keep, p, -step * m * reciprocal(fmaf(r, inv_root_c2, eps)));
+        return r;
     }
 };
 
 __device__ __forceinline__ float warp_max(float v)
 {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    float r;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 
-// N elements of one access of a type
+// Eight elements of a lane as they lie in memory: COUNT accesses of N of them, STRIDE apart.
 template <typename T, int N>
-__device__ __forceinline__ void load(const void* base, long long i, float (&f)[N])
-{
-    constexpr int PER = N * sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
+struct Raw8 {
+    static constexpr int COUNT = 8 / N, STRIDE = 32 * N, PER = N * sizeof(T) > 16 ? 16 / (int)sizeof(T) : N, PIECES = N / PER;
+    Raw<T, PER> raw[COUNT][PIECES];
+    __device__ __forceinline__ void load(const T* p, long long left)              // the first `left` elements of the unit are there
+    {
 #pragma unroll
-    for (int k = 0; k < N / PER; ++k) {
-        float part[PER];
-        unpack<T, PER>(gldv<Raw<T, PER>>(static_cast<const T*>(base) + i + k * PER), part);
+        for (int k = 0; k < COUNT; ++k)
 #pragma unroll
-        for (int j = 0; j < PER; ++j) f[k * PER + j] = part[j];
-    }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store(void* base, long long i, const float (&f)[N])
-{
-    constexpr int PER = N * sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
-#pragma unroll
-    for (int k = 0; k < N / PER; ++k) {
-        float part[PER];
-#pragma unroll
-        for (int j = 0; j < PER; ++j) part[j] = f[k * PER + j];
-        gstv(static_cast<T*>(base) + i + k * PER, pack<T, PER>(part));
-    }
-}
-
-// One unit of 256 elements from `first`: COUNT accesses of N elements to a lane, `stride` elements apart.  MASK: the
-// unit reaches past the tensor's end.
-template <typename P, typename G, bool SMALL, bool MASTER, int N, bool MASK>
-__device__ __forceinline__ void unit(const Entry& e, long long first, int lane, const Step& step)
-{
-    constexpr int COUNT = 8 / N, STRIDE = 32 * N;
-    float p[COUNT][N], g[COUNT][N], m[COUNT][N], v[COUNT][N];
-    float ms = 0.0f, vs = 0.0f;
-    const long long block = first / kUnit;
-    if constexpr (SMALL) { ms = gld(e.ms + block); vs = gld(e.vs + block); }
-#pragma unroll
-    for (int k = 0; k < COUNT; ++k) {
-        const long long i = first + k * STRIDE + lane * N;
-        if (MASK && i >= e.n) {                            // N == 1 there
-#pragma unroll
-            for (int j = 0; j < N; ++j) p[k][j] = g[k][j] = m[k][j] = v[k][j] = 0.0f;
-            continue;
-        }
-        if constexpr (MASTER) load<float, N>(e.w, i, p[k]);
-        else load<P, N>(e.p, i, p[k]);
-        load<G, N>(e.g, i, g[k]);
-        if constexpr (SMALL) {
-            unpack_e4m3<N>(gldv<typename RawOf<N>::type>(static_cast<const uint8_t*>(e.m) + i), m[k]);
-            unpack_e4m3<N>(gldv<typename RawOf<N>::type>(static_cast<const uint8_t*>(e.v) + i), v[k]);
-#pragma unroll
-            for (int j = 0; j < N; ++j) { m[k][j] *= ms; v[k][j] *= vs; v[k][j] *= v[k][j]; }
-        } else {
-            load<float, N>(e.m, i, m[k]);
-            load<float, N>(e.v, i, v[k]);
-        }
-    }
-    float m_max = 0.0f, v_max = 0.0f;
-#pragma unroll
-    for (int k = 0; k < COUNT; ++k) {
-        const long long i = first + k * STRIDE + lane * N;
-#pragma unroll
-        for (int j = 0; j < N; ++j) step(p[k][j], g[k][j], m[k][j], v[k][j]);
-        if (MASK && i >= e.n) continue;
-        if constexpr (MASTER) store<float, N>(e.w, i, p[k]);
-        store<P, N>(e.p, i, p[k]);
-        if constexpr (SMALL) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                v[k][j] = sqrtf(v[k][j]);
-                m_max = max_nan(m_max, fabsf(m[k][j]));
-                v_max = max_nan(v_max, v[k][j]);
+            for (int i = 0; i < PIECES; ++i) {
+                raw[k][i] = Raw<T, PER>{};
+                if (k * STRIDE < left) raw[k][i] = gldv<Raw<T, PER>>(p + k * STRIDE + i * PER);
             }
-        } else {
-            store<float, N>(e.m, i, m[k]);
-            store<float, N>(e.v, i, v[k]);
+    }
+    __device__ __forceinline__ void get(int k, float (&f)[N]) const
+    {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            float part[PER];
+            unpack<T, PER>(raw[k][i], part);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) f[i * PER + j] = part[j];
         }
     }
-    if constexpr (SMALL) {
-        ms = max_nan(warp_max(m_max) / kE4m3Max, kScaleMin);
-        vs = max_nan(warp_max(v_max) / kE4m3Max, kScaleMin);
-        const float mi = 1.0f / ms, vi = 1.0f / vs;
-        constexpr float kSmallest = 0.001953125f;          // 2^-9
-        if (lane == 0) { gst(e.ms + block, ms); gst(e.vs + block, vs); }
+};
+template <typename T, int N>
+__device__ __forceinline__ void store(T* p, const float (&f)[N])
+{
+    constexpr int PER = N * sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N / PER; ++i) {
+        float part[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) part[j] = f[i * PER + j];
+        gstv(p + i * PER, pack<T, PER>(part));
+    }
+}
+
+// One unit of 256 elements of a warp: loaded first, so that the next one's loads are on their way while this one is worked on.
+template <typename P, typename G, bool SMALL, bool MASTER, int N>
+struct Unit {
+    using S = std::conditional_t<SMALL, uint8_t, float>;
+    using W = std::conditional_t<MASTER, float, P>;
+    static constexpr int COUNT = 8 / N, STRIDE = 32 * N;
+    Raw8<W, N> w;
+    Raw8<G, N> g;
+    Raw8<S, N> m, v;
+    float ms, vs;
+    long long at, left;                                    // this lane's first element; how many of the unit's there are from it
+
+    __device__ __forceinline__ void load(const Entry& e, long long first, int lane)
+    {
+        at = first + lane * N;
+        left = N == 1 ? e.n - at : 256;
+        if constexpr (MASTER) w.load(e.w + at, left);
+        else w.load(static_cast<const P*>(e.p) + at, left);
+        g.load(static_cast<const G*>(e.g) + at, left);
+        m.load(static_cast<const S*>(e.m) + at, left);
+        v.load(static_cast<const S*>(e.v) + at, left);
+        if constexpr (SMALL) { ms = gld(e.ms + first / kUnit); vs = gld(e.vs + first / kUnit); }
+    }
+    __device__ __forceinline__ void work(const Entry& e, long long first, int lane, const Step& step)
+    {
+        float m1[COUNT][N], v1[COUNT][N], m_max = 0.0f, v_max = 0.0f;
 #pragma unroll
         for (int k = 0; k < COUNT; ++k) {
-            const long long i = first + k * STRIDE + lane * N;
-            if (MASK && i >= e.n) continue;
+            float p[N], grad[N];
+            w.get(k, p);
+            g.get(k, grad);
+            if constexpr (SMALL) {
+                unpack_e4m3<N>(m.raw[k][0], m1[k]);
+                unpack_e4m3<N>(v.raw[k][0], v1[k]);
+#pragma unroll
+                for (int j = 0; j < N; ++j) { m1[k][j] *= ms; v1[k][j] *= vs; v1[k][j] *= v1[k][j]; }
+            } else {
+                m.get(k, m1[k]);
+                v.get(k, v1[k]);
+            }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                m[k][j] *= mi;
-                v[k][j] = v[k][j] > 0.0f ? max_nan(v[k][j] * vi, kSmallest) : v[k][j];
+                const float r = step(p[j], grad[j], m1[k][j], v1[k][j]);
+                if constexpr (SMALL) v1[k][j] = r;
             }
-            gstv(static_cast<uint8_t*>(e.m) + i, pack_e4m3<N>(m[k]));
-            gstv(static_cast<uint8_t*>(e.v) + i, pack_e4m3<N>(v[k]));
+            if (k * STRIDE < left) {
+                if constexpr (MASTER) store<float, N>(e.w + at + k * STRIDE, p);
+                store<P, N>(static_cast<P*>(e.p) + at + k * STRIDE, p);
+                if constexpr (SMALL) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        m_max = max_nan(m_max, fabsf(m1[k][j]));
+                        v_max = max_nan(v_max, v1[k][j]);
+                    }
+                } else {
+                    store<float, N>(static_cast<float*>(e.m) + at + k * STRIDE, m1[k]);
+                    store<float, N>(static_cast<float*>(e.v) + at + k * STRIDE, v1[k]);
+                }
+            }
+        }
+        if constexpr (SMALL) {
+            const float m_scale = e4m3_scale(warp_max(m_max)), v_scale = e4m3_scale(warp_max(v_max));
+            const float mi = e4m3_inverse(m_scale), vi = e4m3_inverse(v_scale);
+            constexpr float kSmallest = 0.001953125f;      // 2^-9
+            if (lane == 0) { gst(e.ms + first / kUnit, m_scale); gst(e.vs + first / kUnit, v_scale); }
+#pragma unroll
+            for (int k = 0; k < COUNT; ++k) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    m1[k][j] *= mi;
+                    v1[k][j] = v1[k][j] > 0.0f ? max_nan(v1[k][j] * vi, kSmallest) : v1[k][j];
+                }
+                if (k * STRIDE < left) {
+                    gstv(static_cast<uint8_t*>(e.m) + at + k * STRIDE, pack_e4m3<N>(m1[k]));
+                    gstv(static_cast<uint8_t*>(e.v) + at + k * STRIDE, pack_e4m3<N>(v1[k]));
+                }
+            }
         }
     }
+};
+
+template <typename P, typename G, bool SMALL, bool MASTER, int N>
+__device__ __forceinline__ void one_unit(const Entry& e, long long first, int lane, const Step& step)
+{
+    Unit<P, G, SMALL, MASTER, N> u;
+    u.load(e, first, lane);
+    u.work(e, first, lane, step);
 }
 
+// Blocks of an SM: four (64 registers a thread, nothing spilled), six for 16-bit parameters with states in 8 bits, whose
+// lanes have half the bytes under way (64 M bf16 parameters: 122 against 134 us, with a master copy 164 against 167; fp32
+// parameters with states in 8 bits 157 against 171 us at six).
 template <typename P, typename G, bool SMALL, bool MASTER, int MAX>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, SMALL && sizeof(P) == 2 ? 6 : 4)
 adamw_kernel(const __grid_constant__ AdamwParams<MAX> a)
 {
     if (a.skip_device && gld(a.skip_device) != 0.0f) return;
@@ -181,43 +232,37 @@ adamw_kernel(const __grid_constant__ AdamwParams<MAX> a)
         inv_c1 = -1.0f / expm1f(t * a.log_b1);
         inv_c2 = -1.0f / expm1f(t * a.log_b2);
     }
-    const Step step{rate, a.b1, a.b2, a.omb1, a.omb2, a.eps, a.decay, grad_scale, inv_c1, inv_c2};
+    const Step step{a.b1, a.b2, a.omb1, a.omb2, a.eps, 1.0f - rate * a.decay, grad_scale, rate * inv_c1, sqrtf(inv_c2)};
     constexpr int N = sizeof(P) == 4 ? 4 : 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-        int lo = 0, hi = a.count;                          // the last entry that begins at or before this chunk
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.e[mid].first_chunk <= chunk) lo = mid; else hi = mid;
-        }
-        const Entry& e = a.e[lo];
-        const long long begin = (long long)(chunk - e.first_chunk) * kChunk;
-        const long long end = begin + kChunk < e.n ? begin + kChunk : e.n;
-        for (long long first = begin + warp * kUnit; first < end; first += kThreads / 32 * kUnit) {
-            if (first + kUnit > e.n) unit<P, G, SMALL, MASTER, 1, true>(e, first, lane, step);
-            else if (e.vector) unit<P, G, SMALL, MASTER, N, false>(e, first, lane, step);
-            else unit<P, G, SMALL, MASTER, 1, false>(e, first, lane, step);
-        }
+    int lo = 0, hi = a.count;                              // the last entry that begins at or before this block's elements
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.e[mid].first_block <= (int)blockIdx.x) lo = mid; else hi = mid;
     }
+    const Entry& e = a.e[lo];
+    const long long first = (long long)((int)blockIdx.x - e.first_block) * kElements + warp * kUnit;
+    if (first >= e.n) return;
+    if (e.vector && first + kUnit <= e.n) one_unit<P, G, SMALL, MASTER, N>(e, first, lane, step);
+    else one_unit<P, G, SMALL, MASTER, 1>(e, first, lane, step);
 }
 
 template <typename P, typename G, bool SMALL, bool MASTER>
-int launch(cudaStream_t s, AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>& a, const DeviceInfo& di)
+int launch(cudaStream_t s, AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>& a)
 {
-    const unsigned grid = (unsigned)std::min<long long>(a.chunks, (long long)di.sm_count * 8);
-    adamw_kernel<P, G, SMALL, MASTER, PXE_ADAMW_TENSORS_PER_LAUNCH><<<grid, kThreads, 0, s>>>(a);
+    adamw_kernel<P, G, SMALL, MASTER, PXE_ADAMW_TENSORS_PER_LAUNCH><<<(unsigned)a.blocks, kThreads, 0, s>>>(a);
     PXE_LAUNCH_OK("adamw_kernel");
     return PXE_OK;
 }
 
 template <typename P, typename G>
-int launch(cudaStream_t s, AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>& a, const DeviceInfo& di, bool small, bool master)
+int launch(cudaStream_t s, AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>& a, bool small, bool master)
 {
     if constexpr (sizeof(P) == 4) {
-        return small ? launch<P, G, true, false>(s, a, di) : launch<P, G, false, false>(s, a, di);
+        return small ? launch<P, G, true, false>(s, a) : launch<P, G, false, false>(s, a);
     } else {
-        if (master) return small ? launch<P, G, true, true>(s, a, di) : launch<P, G, false, true>(s, a, di);
-        return small ? launch<P, G, true, false>(s, a, di) : launch<P, G, false, false>(s, a, di);
+        if (master) return small ? launch<P, G, true, true>(s, a) : launch<P, G, false, true>(s, a);
+        return small ? launch<P, G, true, false>(s, a) : launch<P, G, false, false>(s, a);
     }
 }
 
@@ -291,8 +336,6 @@ extern "C" int pxe_adamw_update(pxe_stream_t stream, const pxe_adamw_desc* dp)
         return set_error(PXE_ERR_CUDA, "adamw_update: %s", e.what());
     }
     if (first) return PXE_OK;                              // nothing to do
-    DeviceInfo di;
-    { const int rc = device_info(&di); if (rc != PXE_OK) return rc; }
     AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH> a;
     a.rate = d.rate; a.b1 = d.beta1; a.b2 = d.beta2; a.omb1 = (float)(1.0 - (double)d.beta1); a.omb2 = (float)(1.0 - (double)d.beta2);
     a.eps = d.eps; a.decay = d.weight_decay; a.grad_scale = d.grad_scale;
@@ -304,29 +347,29 @@ extern "C" int pxe_adamw_update(pxe_stream_t stream, const pxe_adamw_desc* dp)
     int i = 0;
     while (i < d.count) {
         a.count = 0;
-        long long chunks = 0;
+        long long blocks = 0;
         for (; i < d.count && a.count < PXE_ADAMW_TENSORS_PER_LAUNCH; ++i) {
             const pxe_adamw_tensor& t = d.tensors[i];
             if (t.n == 0) continue;
-            const long long mine = (t.n + kChunk - 1) / kChunk;
-            if (chunks + mine > 0x3fffffffLL) break;       // chunk numbers are ints; n <= 2^40 leaves room for one tensor
+            const long long mine = (t.n + kElements - 1) / kElements;
+            if (blocks + mine > 0x3fffffffLL) break;       // (n <= 2^40 leaves room for one tensor)
             Entry& e = a.e[a.count++];
-            e = {t.param, t.grad, t.m, t.v, t.m_scale, t.v_scale, t.master, t.n, (int)chunks, 0};
+            e = {t.param, t.grad, t.m, t.v, t.m_scale, t.v_scale, t.master, t.n, (int)blocks, 0};
             const int per = psize == 4 ? 4 : 8;            // elements per access
             const uintptr_t wide = (uintptr_t)t.param | (uintptr_t)t.master | (small ? 0 : (uintptr_t)t.m | (uintptr_t)t.v);
             e.vector = wide % 16 == 0 && (uintptr_t)t.grad % std::min(16, per * gsize) == 0 && (!small || ((uintptr_t)t.m | (uintptr_t)t.v) % per == 0);
-            chunks += mine;
+            blocks += mine;
         }
         if (a.count == 0) break;
-        a.chunks = (int)chunks;
+        a.blocks = (int)blocks;
         int rc;
         if (d.param_type == PXE_F32)
-            rc = d.grad_type == PXE_F32 ? launch<float, float>(s, a, di, small, master)
-               : d.grad_type == PXE_BF16 ? launch<float, bf16>(s, a, di, small, master) : launch<float, f16>(s, a, di, small, master);
+            rc = d.grad_type == PXE_F32 ? launch<float, float>(s, a, small, master)
+               : d.grad_type == PXE_BF16 ? launch<float, bf16>(s, a, small, master) : launch<float, f16>(s, a, small, master);
         else if (d.param_type == PXE_BF16)
-            rc = d.grad_type == PXE_F32 ? launch<bf16, float>(s, a, di, small, master) : launch<bf16, bf16>(s, a, di, small, master);
+            rc = d.grad_type == PXE_F32 ? launch<bf16, float>(s, a, small, master) : launch<bf16, bf16>(s, a, small, master);
         else
-            rc = d.grad_type == PXE_F32 ? launch<f16, float>(s, a, di, small, master) : launch<f16, f16>(s, a, di, small, master);
+            rc = d.grad_type == PXE_F32 ? launch<f16, float>(s, a, small, master) : launch<f16, f16>(s, a, small, master);
         if (rc != PXE_OK) return rc;
     }
     return PXE_OK;

@@ -11,6 +11,7 @@
 // read.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "pxe_types.cuh"
 
@@ -154,143 +155,119 @@ __device__ __forceinline__ int first_column()
 }
 
 // ---------------------------------------------------------------- forward, row in registers
-// blockDim = (tpr, rows per block); short rows share a warp.  While they fit, weights stay in registers over the block's rows, and the next row is
-// loaded before this one is reduced.
+// blockDim = (tpr, rows per block); short rows share a warp.  One row to a thread and no loop: what hides a row's loads is
+// the SM's other blocks and those that follow (20000 x 1001 bf16: 38 us, against 71 with a loop over rows and the next row
+// loaded ahead, which needs another row's registers and halves the blocks of an SM).
 constexpr int kMaxRowsPerBlock = 8;                        // of more than a warp each
 
-template <typename T, int VEC, int NV, bool Q>
-__global__ void __launch_bounds__(512, NV * VEC <= 8 ? 2 : 1)
+// EARLY: the weights are on their way before the row's sum is known, for launches that leave the SMs half empty (333 x 1023
+// fp32: 2.6 us against 3.7); with many blocks the registers count for more (262144 x 128 bf16: 43.2 us against 41.4).
+template <typename T, int VEC, int NV, bool Q, bool EARLY>
+__global__ void __launch_bounds__(512, NV * VEC <= 16 ? 2 : 1)
 rms_norm_kernel(const NormParams p)
 {
-    constexpr bool KEEP = NV * VEC <= 16, AHEAD = NV * VEC <= 16;
     constexpr int SPAN = 32 * VEC;
-    __shared__ float reds[2][kMaxRowsPerBlock][16], red_max[2][kMaxRowsPerBlock][16];
-    const int slot = blockDim.x > 32 ? threadIdx.y : 0;
+    __shared__ float reds[kMaxRowsPerBlock][16], red_max[kMaxRowsPerBlock][16];
     extern __shared__ unsigned int group_max[];            // Q, groups that no set of lanes of one warp covers: [rpb][groups]
-    const int tpr = blockDim.x, rpb = blockDim.y, C = p.channels, col0 = first_column<VEC, NV>();
-    const T* const px = static_cast<const T*>(p.x) + col0;
-    const T* const pr = p.residual ? static_cast<const T*>(p.residual) + col0 : nullptr;
-    float w[KEEP ? NV : 1][VEC];
-    if constexpr (KEEP) {
+    const int slot = blockDim.x > 32 ? threadIdx.y : 0, C = p.channels, col0 = first_column<VEC, NV>();
+    const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    const int mine = row < p.rows ? C - col0 : 0;          // vector i is there when i * SPAN < mine
+    const T* const x = static_cast<const T*>(p.x) + row * p.xs + col0;
+    const T* const r = static_cast<const T*>(p.residual) + row * p.rs + col0;
+    Raw<T, VEC> xr[NV], rr[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN;
-            if (col < C) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[i]);
+    for (int i = 0; i < NV; ++i) {
+        if (i * SPAN < mine) {
+            xr[i] = gldv<Raw<T, VEC>>(x + i * SPAN);
+            if (p.residual) rr[i] = gldv<Raw<T, VEC>>(r + i * SPAN);
         }
     }
-    Raw<T, VEC> xr[NV], rr[NV];
-    auto load = [&](long long row) {
-        if (row >= p.rows) return;
-        const T* const x = px + row * p.xs;
-        const T* const r = pr + row * p.rs;
+    float w[EARLY ? NV : 1][VEC];
+    if constexpr (EARLY) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN;
-            if (col < C) {
-                xr[i] = gldv<Raw<T, VEC>>(x + i * SPAN);
-                if (pr) rr[i] = gldv<Raw<T, VEC>>(r + i * SPAN);
-            }
-        }
-    };
-    const long long step = (long long)gridDim.x * rpb;
-    if (AHEAD) load((long long)blockIdx.x * rpb + threadIdx.y);
-    int turn = 0;
-    for (long long row0 = (long long)blockIdx.x * rpb; row0 < p.rows; row0 += step, turn ^= 1) {
-        const long long row = row0 + threadIdx.y;
-        const bool active = row < p.rows;
-        T* const h = static_cast<T*>(p.h) + row * p.hs + col0;
-        T* const y = static_cast<T*>(p.y) + row * p.ys + col0;
-        if (!AHEAD) load(row);
-        float v[NV][VEC];
-        float sum = 0.0f;
+        for (int i = 0; i < NV; ++i)
+            if (i * SPAN < mine) load_weight<T, VEC>(p.weight, p.weight_f32, col0 + i * SPAN, w[i]);
+    }
+    float v[NV][VEC];
+    float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN;
-            if (active && col < C) {
-                unpack<T, VEC>(xr[i], v[i]);
-                if (pr) {
-                    float a[VEC];
-                    unpack<T, VEC>(rr[i], a);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) a[j] += v[i][j];
-                    const Raw<T, VEC> raw = pack<T, VEC>(a);
-                    gstv(h + i * SPAN, raw);
-                    unpack<T, VEC>(raw, v[i]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
-            }
-        }
-        if (AHEAD) load(row + step);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) sum = sum_squares<VEC>(v[i], sum);
-        sum = row_reduce<false>(sum, reds[turn][slot]);
-        const float rstd = rsqrtf(sum * p.inv_channels + p.eps);
-        if (p.rstd && active && threadIdx.x == 0) gst(p.rstd + row, rstd);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN;
-            if (active && col < C) {
-                if constexpr (!KEEP) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
-                scale_by<VEC>(v[i], rstd, w[KEEP ? i : 0]);
-                if constexpr (!Q) gstv(y + i * SPAN, pack<T, VEC>(v[i]));
-            }
-        }
-        if constexpr (Q) {
-            uint8_t* const q = p.q + row * p.qs + col0;
-            auto store = [&](int i, float scale) {
-                const float inv = e4m3_inverse(scale);
+    for (int i = 0; i < NV; ++i) {
+        if (i * SPAN < mine) {
+            unpack<T, VEC>(xr[i], v[i]);
+            if (p.residual) {
                 float a[VEC];
+                unpack<T, VEC>(rr[i], a);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) a[j] = v[i][j] * inv;
-                gstv(q + i * SPAN, pack_e4m3<VEC>(a));
-            };
-            if (p.group == 0) {
-                float largest = 0.0f;
+                for (int j = 0; j < VEC; ++j) a[j] += v[i][j];
+                const Raw<T, VEC> raw = pack<T, VEC>(a);
+                gstv(static_cast<T*>(p.h) + row * p.hs + col0 + i * SPAN, raw);
+                unpack<T, VEC>(raw, v[i]);
+            }
+            sum = sum_squares<VEC>(v[i], sum);
+        } else {
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (active && col0 + i * SPAN < C) largest = max_nan(largest, largest_of<VEC>(v[i]));
-                const float scale = e4m3_scale(row_reduce<true>(largest, red_max[turn][slot]));
-                if (active && threadIdx.x == 0) gst(p.scale + row, scale);
+            for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
+        }
+    }
+    sum = row_reduce<false>(sum, reds[slot]);
+    const float rstd = rsqrtf(sum * p.inv_channels + p.eps);
+    if (p.rstd && mine > 0 && threadIdx.x == 0) gst(p.rstd + row, rstd);
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int col = col0 + i * SPAN;
-                    if (active && col < C) store(i, scale);
+    for (int i = 0; i < NV; ++i) {
+        if (i * SPAN < mine) {
+            if constexpr (!EARLY) load_weight<T, VEC>(p.weight, p.weight_f32, col0 + i * SPAN, w[0]);
+            scale_by<VEC>(v[i], rstd, w[EARLY ? i : 0]);
+            if constexpr (!Q) gstv(static_cast<T*>(p.y) + row * p.ys + col0 + i * SPAN, pack<T, VEC>(v[i]));
+        }
+    }
+    if constexpr (Q) {
+        uint8_t* const q = p.q + row * p.qs + col0;
+        auto store = [&](int i, float scale) {
+            const float inv = e4m3_inverse(scale);
+            float a[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) a[j] = v[i][j] * inv;
+            gstv(q + i * SPAN, pack_e4m3<VEC>(a));
+        };
+        if (p.group == 0) {
+            float largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (i * SPAN < mine) largest = max_nan(largest, largest_of<VEC>(v[i]));
+            const float scale = e4m3_scale(row_reduce<true>(largest, red_max[slot]));
+            if (mine > 0 && threadIdx.x == 0) gst(p.scale + row, scale);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (i * SPAN < mine) store(i, scale);
+        } else if (p.group <= 32 * VEC) {                  // a group is group / VEC neighbouring lanes of one warp
+            const int lanes = p.group / VEC;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float m = i * SPAN < mine ? largest_of<VEC>(v[i]) : 0.0f;
+                for (int o = lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                if (i * SPAN < mine) {
+                    const float scale = e4m3_scale(m);
+                    if ((threadIdx.x & (lanes - 1)) == 0) gst(p.scale + row * p.groups + ((col0 + i * SPAN) >> p.group_shift), scale);
+                    store(i, scale);
                 }
-            } else if (p.group <= 32 * VEC) {              // a group is group / VEC neighbouring lanes of one warp
-                const int lanes = p.group / VEC;
+            }
+        } else {                                           // fp32 bits of |y| order as integers do, NaN above everything
+            unsigned int* gm = group_max + threadIdx.y * p.groups;
+            for (int g = threadIdx.x; g < p.groups; g += blockDim.x) gm[g] = 0u;
+            __syncthreads();
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int col = col0 + i * SPAN;
-                    float m = active && col < C ? largest_of<VEC>(v[i]) : 0.0f;
-                    for (int o = lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    if (active && col < C) {
-                        const float scale = e4m3_scale(m);
-                        if ((threadIdx.x & (lanes - 1)) == 0) gst(p.scale + row * p.groups + (col >> p.group_shift), scale);
-                        store(i, scale);
-                    }
-                }
-            } else {                                       // fp32 bits of |y| order as integers do, NaN above everything
-                unsigned int* gm = group_max + threadIdx.y * p.groups;
-                __syncthreads();
-                for (int g = threadIdx.x; g < p.groups; g += tpr) gm[g] = 0u;
-                __syncthreads();
+            for (int i = 0; i < NV; ++i) {
+                const float m = warp_largest(i * SPAN < mine ? largest_of<VEC>(v[i]) : 0.0f);      // (a warp lies within a group)
+                if (i * SPAN < mine && (threadIdx.x & 31) == 0) atomicMax(gm + ((col0 + i * SPAN) >> p.group_shift), __float_as_uint(m));
+            }
+            __syncthreads();
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int col = col0 + i * SPAN;
-                    const float m = warp_largest(active && col < C ? largest_of<VEC>(v[i]) : 0.0f);      // (a warp lies within a group)
-                    if (active && col < C && (threadIdx.x & 31) == 0) atomicMax(gm + (col >> p.group_shift), __float_as_uint(m));
-                }
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int col = col0 + i * SPAN;
-                    if (active && col < C) {
-                        const float scale = e4m3_scale(__uint_as_float(gm[col >> p.group_shift]));
-                        if ((col & (p.group - 1)) == 0) gst(p.scale + row * p.groups + (col >> p.group_shift), scale);
-                        store(i, scale);
-                    }
+            for (int i = 0; i < NV; ++i) {
+                const int col = col0 + i * SPAN;
+                if (i * SPAN < mine) {
+                    const float scale = e4m3_scale(__uint_as_float(gm[col >> p.group_shift]));
+                    if ((col & (p.group - 1)) == 0) gst(p.scale + row * p.groups + (col >> p.group_shift), scale);
+                    store(i, scale);
                 }
             }
         }
@@ -457,7 +434,7 @@ __device__ __forceinline__ void store_partial(const float (&acc)[NV][VEC], float
 }
 
 template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, NV == 1 ? 2 : 1)    // (NV == 1: 262144 x 128 bf16 53 us against 78)
 rms_norm_backward_kernel(const NormBackParams p)
 {
     constexpr bool HOLD = NV * VEC <= 8;
@@ -595,11 +572,13 @@ rms_norm_backward_long_kernel(const NormBackParams p)
     }
 }
 
-// ---------------------------------------------------------------- many rows of whole vectors: a ring of rows in shared memory
-// The forms above wait for one row while they work on another; that leaves too few bytes on their way (a row's chain of
-// load, barrier, reduction and store takes about 1.5 us, whatever it moves).  Here one thread keeps `stages` rows of
-// every input coming in with bulk copies.  A row's barrier in its reduction says that all threads are done with the row
-// before, whose place is then refilled.  Waits are bounded: a copy that never completes leaves NaN behind, not a hang.
+// ---------------------------------------------------------------- backward, many rows of whole vectors: a ring of rows in shared memory
+// A block has to go over many rows (its part of dweight is in its registers), and the form above waits for one row while it
+// works on another: too few bytes are on their way (a row's chain of load, barrier, reduction and store takes about 1.5 us,
+// whatever it moves).  Here one thread keeps `stages` rows of every input coming in with bulk copies.  A row's barrier in
+// its reduction says that all threads are done with the row before, whose place is then refilled.  Waits are bounded: a
+// copy that never completes leaves NaN behind, not a hang.  16384 x 4096 bf16: 82 us, the copy rate, against 91.  (Several short rows to
+// a stage, filled by a warp, were slower than the form above: 44 against 28 us at 8192 x 2048.)
 constexpr int kMaxStages = 8;
 constexpr int kWaitLimit = 1 << 20;
 
@@ -651,125 +630,15 @@ struct Ring {
 
 extern __shared__ __align__(128) unsigned char ring_shared[];
 
-template <typename T, int NV, bool Q>
-__global__ void __launch_bounds__(512)
-rms_norm_ring_kernel(const NormParams p, int stages)
-{
-    constexpr int VEC = 16 / sizeof(T), SPAN = 32 * VEC;
-    constexpr bool KEEP = NV * VEC <= 16;
-    __shared__ float reds[2][16], red_max[2][16];
-    __shared__ unsigned long long full[kMaxStages];
-    const int C = p.channels, col0 = first_column<VEC, NV>(), bytes = C * (int)sizeof(T), inputs = p.residual ? 2 : 1;
-    const Ring ring{ring_shared, full, stages, bytes * inputs};
-    ring.init();
-    auto fill = [&](int stage, long long row) {
-        const void* const src[2] = {static_cast<const T*>(p.x) + row * p.xs, static_cast<const T*>(p.residual) + row * p.rs};
-        ring.fill<2>(stage, src, inputs, bytes);
-    };
-    const long long step = gridDim.x;
-    if (threadIdx.x == 0)
-        for (int i = 0; i < stages; ++i)
-            if (blockIdx.x + i * step < p.rows) fill(i, blockIdx.x + i * step);
-    float w[KEEP ? NV : 1][VEC];
-    if constexpr (KEEP) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN;
-            if (col < C) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[i]);
-        }
-    }
-    int stage = 0, parity = 0, turn = 0;
-    for (long long row = blockIdx.x; row < p.rows; row += step, turn ^= 1) {
-        const bool arrived = ring.wait(stage, parity);
-        const unsigned char* const at = ring.data + stage * ring.stage_bytes + col0 * (int)sizeof(T);
-        const unsigned char* const at2 = at + bytes;
-        T* const h = static_cast<T*>(p.h) + row * p.hs + col0;
-        T* const y = static_cast<T*>(p.y) + row * p.ys + col0;
-        uint8_t* const q = p.q + row * p.qs + col0;
-        float v[NV][VEC];
-        float sum = arrived ? 0.0f : __int_as_float(0x7fffffff);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN;
-            if (col < C) {
-                unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + i * SPAN * (int)sizeof(T)), v[i]);
-                if (p.residual) {
-                    float a[VEC];
-                    unpack<T, VEC>(ring.read<Raw<T, VEC>>(at2 + i * SPAN * (int)sizeof(T)), a);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) a[j] += v[i][j];
-                    const Raw<T, VEC> raw = pack<T, VEC>(a);
-                    gstv(h + i * SPAN, raw);
-                    unpack<T, VEC>(raw, v[i]);
-                }
-                sum = sum_squares<VEC>(v[i], sum);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
-            }
-        }
-        sum = row_reduce<false>(sum, reds[turn]);
-        const int before = stage == 0 ? stages - 1 : stage - 1;
-        if (threadIdx.x == 0 && row != blockIdx.x && row + (stages - 1) * step < p.rows) fill(before, row + (stages - 1) * step);
-        const float rstd = rsqrtf(sum * p.inv_channels + p.eps);
-        if (p.rstd && threadIdx.x == 0) gst(p.rstd + row, rstd);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN;
-            if (col < C) {
-                if constexpr (!KEEP) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
-                scale_by<VEC>(v[i], rstd, w[KEEP ? i : 0]);
-                if constexpr (!Q) gstv(y + i * SPAN, pack<T, VEC>(v[i]));
-            }
-        }
-        if constexpr (Q) {
-            auto store = [&](int i, float scale) {
-                const float inv = e4m3_inverse(scale);
-                float a[VEC];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) a[j] = v[i][j] * inv;
-                gstv(q + i * SPAN, pack_e4m3<VEC>(a));
-            };
-            if (p.group == 0) {
-                float largest = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (col0 + i * SPAN < C) largest = max_nan(largest, largest_of<VEC>(v[i]));
-                const float scale = e4m3_scale(row_reduce<true>(largest, red_max[turn]));
-                if (threadIdx.x == 0) gst(p.scale + row, scale);
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int col = col0 + i * SPAN;
-                    if (col < C) store(i, scale);
-                }
-            } else {                                       // a group is group / VEC neighbouring lanes of one warp
-                const int lanes = p.group / VEC;
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int col = col0 + i * SPAN;
-                    float m = col < C ? largest_of<VEC>(v[i]) : 0.0f;
-                    for (int o = lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    if (col < C) {
-                        const float scale = e4m3_scale(m);
-                        if ((threadIdx.x & (lanes - 1)) == 0) gst(p.scale + row * p.groups + (col >> p.group_shift), scale);
-                        store(i, scale);
-                    }
-                }
-            }
-        }
-        if (++stage == stages) { stage = 0; parity ^= 1; }
-    }
-}
-
-template <typename T, int NV>
-__global__ void __launch_bounds__(512)
+template <typename T>
+__global__ void __launch_bounds__(1024)
 rms_norm_backward_ring_kernel(const NormBackParams p, int stages)
 {
-    constexpr int VEC = 16 / sizeof(T), SPAN = 32 * VEC;
-    constexpr bool HOLD = NV * VEC <= 8;
-    __shared__ float reds[2][16];
+    constexpr int VEC = 16 / sizeof(T);                    // a thread holds one vector of the row
+    __shared__ float reds[2][32];
     __shared__ unsigned long long full[kMaxStages];
-    const int C = p.channels, col0 = first_column<VEC, NV>(), bytes = C * (int)sizeof(T), inputs = p.dres ? 3 : 2;
+    const int C = p.channels, col = threadIdx.x * VEC, bytes = C * (int)sizeof(T), inputs = p.dres ? 3 : 2;
+    const bool there = col < C;
     const Ring ring{ring_shared, full, stages, bytes * inputs};
     ring.init();
     auto fill = [&](int stage, long long row) {
@@ -780,88 +649,78 @@ rms_norm_backward_ring_kernel(const NormBackParams p, int stages)
     if (threadIdx.x == 0)
         for (int i = 0; i < stages; ++i)
             if (blockIdx.x + i * step < p.rows) fill(i, blockIdx.x + i * step);
-    float acc[NV][VEC], w[HOLD ? NV : 1][VEC];
+    float acc[1][VEC], w[VEC], u[VEC], h[VEC];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[i][j] = 0.0f;
-    if constexpr (HOLD) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN;
-            if (col < C) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[i]);
-        }
-    }
+    for (int j = 0; j < VEC; ++j) acc[0][j] = u[j] = h[j] = 0.0f;
+    if (there) load_weight<T, VEC>(p.weight, p.weight_f32, col, w);
     float next_rstd = gld(p.rstd + blockIdx.x);            // (there are at least two rows for each block)
     int stage = 0, parity = 0, turn = 0;
     for (long long row = blockIdx.x; row < p.rows; row += step, turn ^= 1) {
         const float rstd = next_rstd;
         if (row + step < p.rows) next_rstd = gld(p.rstd + row + step);
         const bool arrived = ring.wait(stage, parity);
-        const unsigned char* const at = ring.data + stage * ring.stage_bytes + col0 * (int)sizeof(T);
-        const unsigned char* const at2 = at + bytes;
-        const unsigned char* const at3 = at2 + bytes;
-        T* const dx = static_cast<T*>(p.dx) + row * p.dxs + col0;
-        float u[HOLD ? NV : 1][VEC], h[HOLD ? NV : 1][VEC];
+        const unsigned char* const at = ring.data + stage * ring.stage_bytes + col * (int)sizeof(T);
         float dot = arrived ? 0.0f : __int_as_float(0x7fffffff);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN, k = HOLD ? i : 0;
-            if (col < C) {
-                if constexpr (!HOLD) load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
-                unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + i * SPAN * (int)sizeof(T)), u[k]);
-                unpack<T, VEC>(ring.read<Raw<T, VEC>>(at2 + i * SPAN * (int)sizeof(T)), h[k]);
-                dot = first_pass<T, VEC>(u[k], h[k], w[k], rstd, acc[i], dot);
-            }
+        if (there) {
+            unpack<T, VEC>(ring.read<Raw<T, VEC>>(at), u);
+            unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + bytes), h);
+            dot = first_pass<T, VEC>(u, h, w, rstd, acc[0], dot);
         }
         dot = row_reduce<false>(dot, reds[turn]);
         const int before = stage == 0 ? stages - 1 : stage - 1;
         if (threadIdx.x == 0 && row != blockIdx.x && row + (stages - 1) * step < p.rows) fill(before, row + (stages - 1) * step);
-        const float factor = -(dot * p.inv_channels * rstd * rstd * rstd);
+        if (there) {
+            float res[VEC];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = col0 + i * SPAN, k = HOLD ? i : 0;
-            if (col < C) {
-                if constexpr (!HOLD) {
-                    load_weight<T, VEC>(p.weight, p.weight_f32, col, w[0]);
-                    unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + i * SPAN * (int)sizeof(T)), u[0]);
-                    unpack<T, VEC>(ring.read<Raw<T, VEC>>(at2 + i * SPAN * (int)sizeof(T)), h[0]);
-                    times<T, VEC>(u[0], w[0]);
-                }
-                float res[VEC];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) res[j] = 0.0f;
-                if (p.dres) unpack<T, VEC>(ring.read<Raw<T, VEC>>(at3 + i * SPAN * (int)sizeof(T)), res);
-                second_pass<VEC>(u[k], h[k], res, rstd, factor);
-                gstv(dx + i * SPAN, pack<T, VEC>(u[k]));
-            }
+            for (int j = 0; j < VEC; ++j) res[j] = 0.0f;
+            if (p.dres) unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + 2 * bytes), res);
+            second_pass<VEC>(u, h, res, rstd, -(dot * p.inv_channels * rstd * rstd * rstd));
+            gstv(static_cast<T*>(p.dx) + row * p.dxs + col, pack<T, VEC>(u));
         }
         if (++stage == stages) { stage = 0; parity ^= 1; }
     }
-    if (p.partial == nullptr) return;
-    store_partial<VEC, NV>(acc, p.partial + (long long)blockIdx.x * C, C, col0, nullptr);
+    if (p.partial) store_partial<VEC, 1>(acc, p.partial + (long long)blockIdx.x * C, C, col, nullptr);
 }
 
-// dweight[c] = the sum of column c over the workspace's rows: 16 columns by 64 row groups to a block, each group's rows and
-// then the groups in order.  Launched while the kernel that fills the workspace still runs; it waits for that one's end.
-__global__ void __launch_bounds__(1024)
+// dweight[c] = the sum of column c over the workspace's rows.  A block takes 32 columns, eight threads of four columns side
+// by side (one 128-byte line of a row) and 128 rows at a time; then each warp's four row groups and the 32 warps are added
+// in order.  Launched while the kernel that fills the workspace still runs; it waits for that one's end.
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads)
 rms_norm_dweight_kernel(const float* partial, int parts, int channels, float* dweight, int accumulate)
 {
-    __shared__ float part[64][17];
-    const int c = blockIdx.x * 16 + threadIdx.x;
-    float sum = 0.0f;
+    __shared__ float part[32][33];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, c = blockIdx.x * 32 + (t & 7) * 4;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     cudaGridDependencySynchronize();
-    if (c < channels) {
-#pragma unroll 10
-        for (int r = threadIdx.y; r < parts; r += 64) sum += gld(partial + (long long)r * channels + c);
-    }
-    part[threadIdx.y][threadIdx.x] = sum;
-    __syncthreads();
-    if (threadIdx.y == 0 && c < channels) {
+    if (channels % 4 == 0) {
+        if (c < channels) {
+#pragma unroll 5
+            for (int r = t >> 3; r < parts; r += kSumThreads / 8) {
+                float f[4];
+                unpack<float, 4>(gldv<uint4>(partial + (long long)r * channels + c), f);
 #pragma unroll
-        for (int y = 1; y < 64; ++y) sum += part[y][threadIdx.x];
-        gst(dweight + c, accumulate ? gld(dweight + c) + sum : sum);
+                for (int j = 0; j < 4; ++j) sum[j] += f[j];
+            }
+        }
+    } else {
+        for (int r = t >> 3; r < parts; r += kSumThreads / 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < channels) sum[j] += gld(partial + (long long)r * channels + c + j);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 8);
+        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 16);
+        if (lane < 8) part[warp][lane * 4 + j] = sum[j];
+    }
+    __syncthreads();
+    float total = part[lane][warp];                        // column `warp` of the block: a lane for each warp's sum
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int column = blockIdx.x * 32 + warp;
+    if (lane == 0 && column < channels) gst(dweight + column, accumulate ? gld(dweight + column) + total : total);
 }
 
 // ---------------------------------------------------------------- host
@@ -880,14 +739,15 @@ struct Layout {
 };
 
 // Threads and registers for rows of `channels`.  What a row costs whatever its length (two trees of shuffles, a barrier)
-// wants few threads with much each: rows that a warp holds with up to eight accesses or 32 bytes of a tensor a lane (forward,
-// one whole vector) take a warp (or the power of two of its lanes that is enough), longer ones as many threads with as much, up to 512, then with
-// 64 bytes.  With `few` rows (less than one for each SM), where nothing but a row's own time counts, one access up to 512
-// threads; backward, where a thread holds three tensors and a sum for each element, up to 8 elements first.
+// wants few threads with much each: rows that a warp holds with up to eight accesses or 32 bytes of a tensor a lane take a
+// warp (or the power of two of its lanes that is enough); longer ones 128 threads with up to four vectors, then as many
+// threads as they need, up to 512 (16384 x 4096 bf16: 82 us with four vectors, 91 with two).  With `few` rows (less than
+// one for each SM), where nothing but a row's own time counts, one access up to 512 threads; backward, where a thread
+// holds three tensors and a sum for each element, 8 elements first.
 Layout layout_for(int vec, int size, int channels, bool few, bool backward)
 {
     Layout l{vec, 1, 32, 1};
-    const int vecs = (channels + vec - 1) / vec, most = vec * size == 16 && !backward ? 1 : std::min(8, 32 / (vec * size));
+    const int vecs = (channels + vec - 1) / vec, most = backward ? std::min(8, 8 / vec) : std::min(8, 32 / (vec * size));
     if (vecs <= 32) {
         l.tpr = 1;
         while (l.tpr < vecs) l.tpr *= 2;
@@ -900,7 +760,7 @@ Layout layout_for(int vec, int size, int channels, bool few, bool backward)
             l.rpb = 8;
             return l;
         }
-        if (backward) l.nv = std::min(most, std::max(1, 8 / vec));
+        while (!backward && l.nv < 4 && l.nv * 128 < vecs) l.nv *= 2;
     }
     while (l.nv * 512 < vecs) l.nv *= 2;
     if (l.nv > 8 || l.nv * vec * size > 64) {
@@ -913,20 +773,19 @@ Layout layout_for(int vec, int size, int channels, bool few, bool backward)
     return l;
 }
 
-// The ring form takes rows of 2 to 32 KB in whole vectors, when there are enough of them to fill the card: as many threads
-// as the row needs with one vector each, then two, up to 512 threads with four; 1024 threads to an SM (512 where a thread
-// holds four), and the stages that seven eighths of the shared memory hold.
+// The ring form takes rows of 2 to 16 KB in whole vectors, when there are enough of them to fill the card: a thread for each
+// vector, 1024 threads to an SM, and the stages that seven eighths of the shared memory hold.  (Rows of 32 KB leave room for
+// two stages: 121 us against 113 for the form above at 4096 x 16384 bf16.)
 struct RingLayout {
-    int nv, tpr, blocks_per_sm, stages;
+    int threads, blocks_per_sm, stages;
     size_t shared;
 };
 bool ring_layout(int size, int channels, int inputs, long long rows, const DeviceInfo& di, RingLayout* l)
 {
-    const int bytes = channels * size, vecs = bytes / 16;
-    if (bytes < 2048 || bytes > 32768) return false;
-    l->nv = vecs <= 256 ? 1 : vecs <= 1024 ? 2 : 4;
-    l->tpr = ((vecs + l->nv - 1) / l->nv + 31) / 32 * 32;
-    l->blocks_per_sm = std::max(1, (l->nv == 4 ? 512 : 1024) / l->tpr);
+    const int bytes = channels * size;
+    if (bytes < 2048 || bytes > 16384) return false;
+    l->threads = (bytes / 16 + 31) / 32 * 32;
+    l->blocks_per_sm = 1024 / l->threads;
     if (rows < 2LL * di.sm_count * l->blocks_per_sm) return false;
     l->stages = (int)std::min<long long>(kMaxStages, (long long)di.max_smem_optin * 7 / 8 / l->blocks_per_sm / (bytes * inputs));
     l->shared = (size_t)l->stages * bytes * inputs;
@@ -943,35 +802,14 @@ int allow_shared(K kernel, int device, int bytes, std::atomic<unsigned long long
     return PXE_OK;
 }
 
-template <typename T, int NV, bool Q>
-int launch_norm_ring(cudaStream_t s, const NormParams& p, const RingLayout& l, const DeviceInfo& di, int device)
-{
-    static std::atomic<unsigned long long> done{0};
-    { const int rc = allow_shared(rms_norm_ring_kernel<T, NV, Q>, device, di.max_smem_optin - 4096, done); if (rc != PXE_OK) return rc; }
-    rms_norm_ring_kernel<T, NV, Q><<<(unsigned)(di.sm_count * l.blocks_per_sm), l.tpr, l.shared, s>>>(p, l.stages);
-    PXE_LAUNCH_OK("rms_norm_ring_kernel");
-    return PXE_OK;
-}
-template <typename T, bool Q>
-int launch_norm_ring(cudaStream_t s, const NormParams& p, const RingLayout& l, const DeviceInfo& di, int device)
-{
-    return l.nv == 1 ? launch_norm_ring<T, 1, Q>(s, p, l, di, device) : l.nv == 2 ? launch_norm_ring<T, 2, Q>(s, p, l, di, device)
-                                                                                   : launch_norm_ring<T, 4, Q>(s, p, l, di, device);
-}
-template <typename T, int NV>
-int launch_backward_ring(cudaStream_t s, const NormBackParams& p, const RingLayout& l, const DeviceInfo& di, int device)
-{
-    static std::atomic<unsigned long long> done{0};
-    { const int rc = allow_shared(rms_norm_backward_ring_kernel<T, NV>, device, di.max_smem_optin - 4096, done); if (rc != PXE_OK) return rc; }
-    rms_norm_backward_ring_kernel<T, NV><<<(unsigned)(di.sm_count * l.blocks_per_sm), l.tpr, l.shared, s>>>(p, l.stages);
-    PXE_LAUNCH_OK("rms_norm_backward_ring_kernel");
-    return PXE_OK;
-}
 template <typename T>
 int launch_backward_ring(cudaStream_t s, const NormBackParams& p, const RingLayout& l, const DeviceInfo& di, int device)
 {
-    return l.nv == 1 ? launch_backward_ring<T, 1>(s, p, l, di, device) : l.nv == 2 ? launch_backward_ring<T, 2>(s, p, l, di, device)
-                                                                                    : launch_backward_ring<T, 4>(s, p, l, di, device);
+    static std::atomic<unsigned long long> done{0};
+    { const int rc = allow_shared(rms_norm_backward_ring_kernel<T>, device, di.max_smem_optin - 4096, done); if (rc != PXE_OK) return rc; }
+    rms_norm_backward_ring_kernel<T><<<(unsigned)(di.sm_count * l.blocks_per_sm), l.threads, l.shared, s>>>(p, l.stages);
+    PXE_LAUNCH_OK("rms_norm_backward_ring_kernel");
+    return PXE_OK;
 }
 
 template <typename T, int VEC, bool Q>
@@ -985,16 +823,20 @@ int launch_norm(cudaStream_t s, const NormParams& p, const Layout& l, const Devi
         return PXE_OK;
     }
     const long long blocks = (p.rows + l.rpb - 1) / l.rpb;
-    const int threads = l.tpr * l.rpb;
-    const unsigned grid = (unsigned)std::min<long long>(blocks, (long long)di.sm_count * std::max(1, 2048 / threads));
+    PXE_REQUIRE(blocks <= 0x7fffffffLL, "rms_norm: too many rows");
     const size_t smem = Q && p.group > 32 * VEC ? group_bytes * l.rpb : 0;
     const dim3 block(l.tpr, l.rpb);
+    auto launch = [&](auto nv) {
+        constexpr int NV = decltype(nv)::value;
+        if (NV * VEC <= 16 && blocks <= 4LL * di.sm_count) rms_norm_kernel<T, VEC, NV, Q, NV * VEC <= 16><<<(unsigned)blocks, block, smem, s>>>(p);
+        else rms_norm_kernel<T, VEC, NV, Q, false><<<(unsigned)blocks, block, smem, s>>>(p);
+    };
     switch (l.nv) {
-    case 1: rms_norm_kernel<T, VEC, 1, Q><<<grid, block, smem, s>>>(p); break;
-    case 2: rms_norm_kernel<T, VEC, 2, Q><<<grid, block, smem, s>>>(p); break;
-    case 4: rms_norm_kernel<T, VEC, 4, Q><<<grid, block, smem, s>>>(p); break;
+    case 1: launch(std::integral_constant<int, 1>{}); break;
+    case 2: launch(std::integral_constant<int, 2>{}); break;
+    case 4: launch(std::integral_constant<int, 4>{}); break;
     default:
-        if constexpr (VEC <= 2) rms_norm_kernel<T, VEC, 8, Q><<<grid, block, smem, s>>>(p);
+        if constexpr (VEC <= 2) launch(std::integral_constant<int, 8>{});
         break;
     }
     PXE_LAUNCH_OK("rms_norm_kernel");
@@ -1091,14 +933,6 @@ extern "C" int pxe_rms_norm(pxe_stream_t stream, const pxe_rms_norm_desc* dp)
     DeviceInfo di;
     { const int rc = device_info(&di); if (rc != PXE_OK) return rc; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    RingLayout rl;
-    if (vec * size == 16 && ring_layout(size, C, d.residual ? 2 : 1, d.rows, di, &rl)) {
-        int device = 0;
-        PXE_CUDA_OK(cudaGetDevice(&device));
-        if (d.type == PXE_F32) return d.q ? launch_norm_ring<float, true>(s, p, rl, di, device) : launch_norm_ring<float, false>(s, p, rl, di, device);
-        if (d.type == PXE_BF16) return d.q ? launch_norm_ring<bf16, true>(s, p, rl, di, device) : launch_norm_ring<bf16, false>(s, p, rl, di, device);
-        return d.q ? launch_norm_ring<f16, true>(s, p, rl, di, device) : launch_norm_ring<f16, false>(s, p, rl, di, device);
-    }
     const Layout l = layout_for(vec, size, C, d.rows < di.sm_count, false);
 #define PXE_NORM_VEC(T, V) return d.q ? launch_norm<T, V, true>(s, p, l, di) : launch_norm<T, V, false>(s, p, l, di)
     if (d.type == PXE_F32) { if (vec == 4) PXE_NORM_VEC(float, 4); PXE_NORM_VEC(float, 1); }
@@ -1186,8 +1020,8 @@ extern "C" int pxe_rms_norm_backward(pxe_stream_t stream, const pxe_rms_norm_bac
     }
     if (rc != PXE_OK || !d.dweight) return rc;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((C + 15) / 16);
-    cfg.blockDim = dim3(16, 64);
+    cfg.gridDim = dim3((C + 31) / 32);
+    cfg.blockDim = dim3(kSumThreads);
     cfg.stream = s;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
