@@ -310,7 +310,7 @@ __device__ __forceinline__ uint32_t sort_descending(uint32_t v)
 }
 
 constexpr int kCandidates = 1024;                          // of a block
-constexpr int kBlocks = 4, kBlocksTop = 3;                 // resident on an SM (256 threads each)
+constexpr int kBlocks = 8;                                 // of 256 threads on an SM: 32 registers a thread, and no loads ahead
 constexpr int kSelected = 64;                              // threads of a block whose elements are read again
 
 template <int THREADS>
@@ -487,11 +487,10 @@ __device__ __forceinline__ void store_top(const ProbsParams& p, long long row, i
 }
 
 template <typename T, int THREADS, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, TOP ? kBlocksTop : kBlocks)
+__global__ void __launch_bounds__(THREADS, kBlocks)
 log_probs_kernel(const ProbsParams p)
 {
     constexpr int VEC = RowView<T>::VEC;
-    constexpr bool AHEAD = !TOP && !CLUSTER;               // the next row's first batch is under way while this one is joined
     namespace cg = cooperative_groups;
     __shared__ Part parts[THREADS / 32];
     __shared__ Part shared_part;
@@ -499,52 +498,26 @@ log_probs_kernel(const ProbsParams p)
     __shared__ std::conditional_t<TOP && CLUSTER, unsigned long long[8 * kMaxTop], NoTop> lists;
     const int t = threadIdx.x;
     const int ranks = CLUSTER ? p.cluster : 1, rank = CLUSTER ? (int)(blockIdx.x % p.cluster) : 0;
-    const long long groups = gridDim.x / ranks;
-    auto target_at = [&](long long row) -> long long { return row >= p.rows ? -1 : p.target ? target_of(p.target, p.target64, row) : 0; };
-    auto slice_at = [&](long long row) {
-        Slice<T> s{RowView<T>(static_cast<const T*>(p.x) + row_offset(row, p.inner, p.outer_stride, p.row_stride), p.classes), 0, 0, rank == 0, rank == ranks - 1};
-        const int per = (s.r.nvec + ranks - 1) / ranks;
-        s.v0 = min(rank * per, s.r.nvec);
-        s.v1 = min(s.v0 + per, s.r.nvec);
-        return s;
-    };
-    auto load = [&](uint4 (&raw)[kBatch], const Slice<T>& s, int v) {
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-            if (v + k * THREADS < s.v1) raw[k] = gldv<uint4>(s.r.x + s.r.element(v + k * THREADS));
-    };
-    uint4 next[kBatch];
-    long long row = blockIdx.x / ranks, target = target_at(row);
-    if (row < p.rows && target >= 0) {
-        const Slice<T> s = slice_at(row);
-        load(next, s, s.v0 + t);
-    }
-    while (row < p.rows) {
-        const long long next_row = row + groups, next_target = target_at(next_row);
+    for (long long row = blockIdx.x / ranks; row < p.rows; row += gridDim.x / ranks) {
+        const long long target = p.target ? target_of(p.target, p.target64, row) : 0;
         if (target < 0) {
             if (rank == 0) store_unused(p, row, t);
-            if (next_target >= 0) {
-                const Slice<T> s = slice_at(next_row);
-                load(next, s, s.v0 + t);
-            }
-            row = next_row;
-            target = next_target;
             continue;
         }
-        const Slice<T> s = slice_at(row);
+        Slice<T> s{RowView<T>(static_cast<const T*>(p.x) + row_offset(row, p.inner, p.outer_stride, p.row_stride), p.classes), 0, 0, rank == 0, rank == ranks - 1};
         const RowView<T>& r = s.r;
+        const int per = (r.nvec + ranks - 1) / ranks;
+        s.v0 = min(rank * per, r.nvec);
+        s.v1 = min(s.v0 + per, r.nvec);
         Running sum;
         sum.clear();
-#pragma unroll 2
         for (int first = s.v0; first < s.v1; first += kBatch * THREADS) {
             uint4 raw[kBatch];
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) raw[k] = next[k];
-            if (first + kBatch * THREADS < s.v1) {
-                load(next, s, first + t + kBatch * THREADS);
-            } else if (AHEAD && next_target >= 0) {
-                const Slice<T> after = slice_at(next_row);
-                load(next, after, after.v0 + t);
+            for (int k = 0; k < kBatch; ++k) {
+                constexpr uint32_t none = Word<T>::NONE;
+                raw[k] = make_uint4(none, none, none, none);
+                if (first + t + k * THREADS < s.v1) raw[k] = gldv<uint4>(r.x + r.element(first + t + k * THREADS));
             }
             if (first + kBatch * THREADS <= s.v1) {
                 sum.template add_vectors<T, kBatch>(raw, p.c);
@@ -552,8 +525,6 @@ log_probs_kernel(const ProbsParams p)
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     if (first + k * THREADS >= s.v1) break;
-                    constexpr uint32_t none = Word<T>::NONE;
-                    if (first + t + k * THREADS >= s.v1) raw[k] = make_uint4(none, none, none, none);
                     sum.template add_vectors<T, 1>(raw + k, p.c);
                 }
             }
@@ -621,18 +592,7 @@ log_probs_kernel(const ProbsParams p)
                 if (t < top) store_top(p, row, t, sh.list[t], result);
                 __syncthreads();
             }
-            if (next_target >= 0) {
-                const Slice<T> after = slice_at(next_row);
-                load(next, after, after.v0 + t);
-            }
-        } else if constexpr (CLUSTER) {
-            if (next_target >= 0) {
-                const Slice<T> after = slice_at(next_row);
-                load(next, after, after.v0 + t);
-            }
         }
-        row = next_row;
-        target = next_target;
     }
 }
 
@@ -645,114 +605,99 @@ log_probs_short_kernel(const ProbsParams p)
     constexpr int VEC = RowView<T>::VEC, WARPS = kShortThreads / 32;
     __shared__ std::conditional_t<TOP, unsigned long long[WARPS][kShortCandidates], NoTop> candidates;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // what a lane takes of a row: NB vectors, and one of the single elements in front and behind (at most 2 * (VEC - 1))
-    Raw<T, VEC> next[NB];
-    T next_one = from_f32<T>(0.0f);
-    auto view = [&](long long row) {
-        return RowView<T>(static_cast<const T*>(p.x) + row_offset(row, p.inner, p.outer_stride, p.row_stride), p.classes);
-    };
-    auto single_of = [&](const RowView<T>& r) { return lane < r.head ? lane : r.tail() + lane - r.head; };
-    auto load = [&](long long row) {
-        if (row >= p.rows) return;
-        const RowView<T> r = view(row);
+    const long long row = (long long)blockIdx.x * WARPS + warp;
+    if (row >= p.rows) return;
+    const RowView<T> r(static_cast<const T*>(p.x) + row_offset(row, p.inner, p.outer_stride, p.row_stride), p.classes);
+    // what a lane takes of the row: NB vectors, and one of the single elements in front and behind (at most 2 * (VEC - 1))
+    Raw<T, VEC> raw[NB];
 #pragma unroll
-        for (int k = 0; k < NB; ++k)
-            if (lane + 32 * k < r.nvec) next[k] = gldv<Raw<T, VEC>>(r.x + r.element(lane + 32 * k));
-        const int one = single_of(r);
-        if (one < p.classes) next_one = gld(r.x + one);
-    };
-    const long long step = (long long)gridDim.x * WARPS;
-    long long row = (long long)blockIdx.x * WARPS + warp;
-    load(row);
-    for (; row < p.rows; row += step) {
-        const long long target = p.target ? target_of(p.target, p.target64, row) : 0;
-        const RowView<T> r = view(row);
-        const int one = single_of(r);
-        const bool single = one < p.classes;
-        const float x1 = single ? to_f32<T>(next_one) : -INFINITY;
-        float x[NB][VEC];
+    for (int k = 0; k < NB; ++k)
+        if (lane + 32 * k < r.nvec) raw[k] = gldv<Raw<T, VEC>>(r.x + r.element(lane + 32 * k));
+    const int one = lane < r.head ? lane : r.tail() + lane - r.head;
+    const bool single = one < p.classes;
+    const float x1 = single ? to_f32<T>(gld(r.x + one)) : -INFINITY;
+    const long long target = p.target ? target_of(p.target, p.target64, row) : 0;
+    if (target < 0) {
+        store_unused(p, row, lane);
+        return;
+    }
+    float x[NB][VEC];
 #pragma unroll
-        for (int k = 0; k < NB; ++k) {
-            unpack<T, VEC>(next[k], x[k]);
-            if (lane + 32 * k >= r.nvec) {
+    for (int k = 0; k < NB; ++k) {
+        unpack<T, VEC>(raw[k], x[k]);
+        if (lane + 32 * k >= r.nvec) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) x[k][j] = -INFINITY;
-            }
+            for (int j = 0; j < VEC; ++j) x[k][j] = -INFINITY;
         }
-        load(row + step);
-        if (target < 0) {
-            store_unused(p, row, lane);
-            continue;
-        }
-        float mine = x1;
+    }
+    float mine = x1;
 #pragma unroll
-        for (int k = 0; k < NB; ++k)
+    for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) mine = max_nan(mine, x[k][j]);
-        const float most = warp_max(mine), m = most == -INFINITY ? 0.0f : most;
-        float s = 0.0f, u = 0.0f;
-        auto add = [&](float v) {
-            const float d = distance(v, m, p.c), e = exp2_fast(d);
-            s += e;
-            u = fmaf(e, d, u);
+        for (int j = 0; j < VEC; ++j) mine = max_nan(mine, x[k][j]);
+    const float most = warp_max(mine), m = most == -INFINITY ? 0.0f : most;
+    float s = 0.0f, u = 0.0f;
+    auto add = [&](float v) {
+        const float d = distance(v, m, p.c), e = exp2_fast(d);
+        s += e;
+        u = fmaf(e, d, u);
+    };
+    add(x1);
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) add(x[k][j]);
+    warp_sum(s, u);
+    const float l2s = log2f(s);
+    const RowResult result{m, s, u / s, l2s};
+    if (lane == 0) store_row<T>(p, row, target, r.x, result, l2s);
+    if constexpr (TOP) {
+        const int top = p.top;
+        unsigned long long* cand = candidates[warp];
+        // visit(key, whether it is one) by all lanes together
+        auto visit = [&](auto&& f) {
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) f(x[k][j], r.element(lane + 32 * k) + j, lane + 32 * k < r.nvec);
+            f(x1, one, single);
         };
-        add(x1);
-#pragma unroll
-        for (int k = 0; k < NB; ++k)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) add(x[k][j]);
-        warp_sum(s, u);
-        const float l2s = log2f(s);
-        const RowResult result{m, s, u / s, l2s};
-        if (lane == 0) store_row<T>(p, row, target, r.x, result, l2s);
-        if constexpr (TOP) {
-            const int top = p.top;
-            unsigned long long* cand = candidates[warp];
-            // visit(key, whether it is one) by all lanes together
-            auto visit = [&](auto&& f) {
-#pragma unroll
-                for (int k = 0; k < NB; ++k)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) f(x[k][j], r.element(lane + 32 * k) + j, lane + 32 * k < r.nvec);
-                f(x1, one, single);
-            };
-            const uint32_t least = __shfl_sync(0xffffffffu, sort_descending(lane < r.nvec || single ? order_of(mine) : 0), top - 1);
-            int n = 0;
-            __syncwarp();
-            visit([&](float v, int i, bool there) {
-                const bool is = there && order_of(v) >= least;
-                const unsigned ballot = __ballot_sync(0xffffffffu, is);
-                const int at = n + __popc(ballot & ((1u << lane) - 1));
-                if (is && at < kShortCandidates) cand[at] = key_of(v, i);
-                n += __popc(ballot);
-            });
-            __syncwarp();
-            if (n <= kShortCandidates) {
-                for (int i = lane; i < n; i += 32) {
-                    const unsigned long long key = cand[i];
-                    int place = 0;
-                    for (int j = 0; j < n; ++j) place += cand[j] > key;
-                    if (place < top) store_top(p, row, place, key, result);
-                }
-            } else {                                       // more ties than the list holds: one after the other
-                unsigned long long last = ~0ull;
-                for (int place = 0; place < top; ++place) {
-                    unsigned long long key = 0;
-                    visit([&](float v, int i, bool there) {
-                        const unsigned long long k = key_of(v, i);
-                        if (there && k < last && k > key) key = k;
-                    });
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) {
-                        const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
-                        key = other > key ? other : key;
-                    }
-                    last = key;
-                    if (lane == 0) store_top(p, row, place, last, result);
-                }
+        const uint32_t least = __shfl_sync(0xffffffffu, sort_descending(lane < r.nvec || single ? order_of(mine) : 0), top - 1);
+        int n = 0;
+        __syncwarp();
+        visit([&](float v, int i, bool there) {
+            const bool is = there && order_of(v) >= least;
+            const unsigned ballot = __ballot_sync(0xffffffffu, is);
+            const int at = n + __popc(ballot & ((1u << lane) - 1));
+            if (is && at < kShortCandidates) cand[at] = key_of(v, i);
+            n += __popc(ballot);
+        });
+        __syncwarp();
+        if (n <= kShortCandidates) {
+            for (int i = lane; i < n; i += 32) {
+                const unsigned long long key = cand[i];
+                int place = 0;
+                for (int j = 0; j < n; ++j) place += cand[j] > key;
+                if (place < top) store_top(p, row, place, key, result);
             }
-            __syncwarp();
+        } else {                                       // more ties than the list holds: one after the other
+            unsigned long long last = ~0ull;
+            for (int place = 0; place < top; ++place) {
+                unsigned long long key = 0;
+                visit([&](float v, int i, bool there) {
+                    const unsigned long long k = key_of(v, i);
+                    if (there && k < last && k > key) key = k;
+                });
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
+                    key = other > key ? other : key;
+                }
+                last = key;
+                if (lane == 0) store_top(p, row, place, last, result);
+            }
         }
+        __syncwarp();
     }
 }
 
@@ -868,9 +813,9 @@ int launch_with(cudaStream_t s, const ProbsParams& p, unsigned grid)
 }
 
 template <typename T, int NB>
-int launch_short(cudaStream_t s, const ProbsParams& p, const DeviceInfo& di)
+int launch_short(cudaStream_t s, const ProbsParams& p)
 {
-    const unsigned grid = (unsigned)std::min<long long>((p.rows + 3) / 4, 16LL * di.sm_count);
+    const unsigned grid = (unsigned)((p.rows + 3) / 4);
     if (p.top) log_probs_short_kernel<T, NB, true><<<grid, kShortThreads, 0, s>>>(p);
     else log_probs_short_kernel<T, NB, false><<<grid, kShortThreads, 0, s>>>(p);
     PXE_LAUNCH_OK("log_probs_short_kernel");
@@ -884,29 +829,33 @@ int launch_forward(cudaStream_t s, ProbsParams& p, const DeviceInfo& di)
 {
     const int vecs = p.classes / (16 / (int)sizeof(T));
     p.cluster = 1;
-    if (vecs <= 32) return launch_short<T, 1>(s, p, di);
-    if (vecs <= 64) return launch_short<T, 2>(s, p, di);
-    if (vecs <= 128) return launch_short<T, 4>(s, p, di);
-    if constexpr (sizeof(T) == 4) { if (vecs <= 256) return launch_short<T, 8>(s, p, di); }
-    while (p.cluster < 8 && p.rows * p.cluster * 2 <= (long long)kBlocksTop * di.sm_count && vecs >= p.cluster * 2 * 256) p.cluster *= 2;
+    if (vecs <= 32) return launch_short<T, 1>(s, p);
+    if (vecs <= 64) return launch_short<T, 2>(s, p);
+    if (vecs <= 128) return launch_short<T, 4>(s, p);
+    if constexpr (sizeof(T) == 4) { if (vecs <= 256) return launch_short<T, 8>(s, p); }
+    while (p.cluster < 8 && p.rows * p.cluster * 2 <= 2LL * di.sm_count && vecs >= p.cluster * 2 * 256) p.cluster *= 2;
     if (p.cluster > 1) return launch_with<T, 256, true>(s, p, (unsigned)(p.rows * p.cluster));
-    return launch_with<T, 256, false>(s, p, (unsigned)std::min<long long>(p.rows, (long long)(p.top ? kBlocksTop : kBlocks) * di.sm_count));
+    return launch_with<T, 256, false>(s, p, (unsigned)p.rows);
 }
 
-// A warp for rows of up to its 128 vectors, a block for every 1024 vectors of longer ones.
+// A warp for rows of up to 128 vectors, two for rows of up to 256, a block for every 1024 vectors of longer ones.
+template <typename T, int TPR>
+int launch_backward(cudaStream_t s, ProbsBackParams& p, int vecs)
+{
+    p.chunks = std::max(1, (vecs + TPR * kBatch - 1) / (TPR * kBatch));
+    const long long rows = kBackThreads / TPR, blocks = (p.rows * p.chunks + rows - 1) / rows;
+    PXE_REQUIRE(blocks <= 0x7fffffffLL, "log_probs_backward: too many rows");
+    auto kernel = p.dentropy ? log_probs_backward_kernel<T, TPR, true> : log_probs_backward_kernel<T, TPR, false>;
+    kernel<<<(unsigned)blocks, kBackThreads, 0, s>>>(p);
+    PXE_LAUNCH_OK("log_probs_backward_kernel");
+    return PXE_OK;
+}
 template <typename T>
 int launch_backward(cudaStream_t s, ProbsBackParams& p)
 {
     const int vecs = p.classes / (16 / (int)sizeof(T));
-    const int per = vecs <= 32 * kBatch ? 32 * kBatch : kBackThreads * kBatch;
-    p.chunks = std::max(1, (vecs + per - 1) / per);
-    const long long parts = p.rows * p.chunks, blocks = per == 32 * kBatch ? (parts + 7) / 8 : parts;
-    PXE_REQUIRE(blocks <= 0x7fffffffLL, "log_probs_backward: too many rows");
-    auto kernel = per == 32 * kBatch ? (p.dentropy ? log_probs_backward_kernel<T, 32, true> : log_probs_backward_kernel<T, 32, false>)
-                                     : (p.dentropy ? log_probs_backward_kernel<T, kBackThreads, true> : log_probs_backward_kernel<T, kBackThreads, false>);
-    kernel<<<(unsigned)blocks, kBackThreads, 0, s>>>(p);
-    PXE_LAUNCH_OK("log_probs_backward_kernel");
-    return PXE_OK;
+    return vecs <= 32 * kBatch ? launch_backward<T, 32>(s, p, vecs) : vecs <= 64 * kBatch ? launch_backward<T, 64>(s, p, vecs)
+                                                                                           : launch_backward<T, kBackThreads>(s, p, vecs);
 }
 
 // Rows of x or dx: the checked strides, and the span they cover as one row tensor.
