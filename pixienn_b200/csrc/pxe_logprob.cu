@@ -869,9 +869,22 @@ int check_rows(const char* name, const void* ptr, int size, long long rows, long
     PXE_REQUIRE(rows == inner || outer >= (inner - 1) * stride + classes, "%s: outer stride %lld, a group covers %lld", name, outer, (inner - 1) * stride + classes);
     return PXE_OK;
 }
-RowSpan group_span(const void* ptr, int size, long long rows, long long inner, long long outer, long long stride, int classes)
+// What such a tensor covers, in two ways that each cover all of it: its groups, and (where a group is a whole number of rows
+// further) its rows.
+struct Cover {
+    RowSpan groups, rows;
+};
+Cover cover(const void* ptr, int size, long long rows, long long inner, long long outer, long long stride, int classes)
 {
-    return {ptr, rows / inner, outer * size, ((inner - 1) * stride + classes) * size};
+    const RowSpan groups{ptr, rows / inner, outer * size, ((inner - 1) * stride + classes) * size};
+    if (rows != inner && outer % stride != 0) return {groups, groups};
+    const long long lines = (rows / inner - 1) * (outer / stride) + inner;
+    return {groups, {ptr, lines, stride * size, (long long)classes * size}};
+}
+bool conflict(const RowSpan& a, const Cover& b) { return rows_conflict(a, b.groups) && rows_conflict(a, b.rows); }
+bool conflict(const Cover& a, const Cover& b)
+{
+    return rows_conflict(a.groups, b.groups) && rows_conflict(a.rows, b.rows) && rows_conflict(a.groups, b.rows) && rows_conflict(a.rows, b.groups);
 }
 
 }  // namespace
@@ -899,11 +912,18 @@ extern "C" int pxe_log_probs(pxe_stream_t stream, const pxe_log_probs_desc* dp)
     p.classes = d.classes; p.target64 = d.target_is_int64; p.top = d.top; p.c = kLog2e / d.temperature; p.inv_temperature = 1.0f / d.temperature;
     const int size = dtype_bytes(d.type);
     { const int rc = check_rows("log_probs: x", d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes); if (rc != PXE_OK) return rc; }
-    const RowSpan x = group_span(d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes);
+    const Cover x = cover(d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes);
     const struct { const void* ptr; long long bytes; } outs[] = {{d.logp, d.rows * 4}, {d.entropy, d.rows * 4}, {d.stats, d.rows * 12},
                                                                  {d.top_logp, d.rows * d.top * 4}, {d.top_index, d.rows * d.top * 4}};
-    for (const auto& o : outs)
-        PXE_REQUIRE(!o.ptr || (o.ptr != d.x && o.ptr != d.target && !rows_conflict({o.ptr, 1, 0, o.bytes}, x)), "log_probs: an output overlaps an input");
+    const RowSpan target{d.target, 1, 0, d.rows * (d.target_is_int64 ? 8 : 4)};
+    for (const auto& o : outs) {
+        if (!o.ptr) continue;
+        const RowSpan span{o.ptr, 1, 0, o.bytes};
+        PXE_REQUIRE(reinterpret_cast<uintptr_t>(o.ptr) % 4 == 0, "log_probs: an output is not aligned to its elements");
+        PXE_REQUIRE(o.ptr != d.x && o.ptr != d.target && !conflict(span, x) && !rows_conflict(span, target), "log_probs: an output overlaps an input");
+        for (const auto& other : outs)
+            PXE_REQUIRE(&other == &o || !other.ptr || (other.ptr != o.ptr && !rows_conflict(span, {other.ptr, 1, 0, other.bytes})), "log_probs: two outputs overlap");
+    }
     DeviceInfo di;
     { const int rc = device_info(&di); if (rc != PXE_OK) return rc; }
     p.careful = !(p.c > 0.02f && p.c < 1e7f);              // what -inf is held at would count, or overflow
@@ -936,14 +956,14 @@ extern "C" int pxe_log_probs_backward(pxe_stream_t stream, const pxe_log_probs_b
     long long inner = d.inner;
     { const int rc = check_rows("log_probs_backward: x", d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes); if (rc != PXE_OK) return rc; }
     { const int rc = check_rows("log_probs_backward: dx", d.dx, size, d.rows, inner, p.dx_outer_stride, p.dx_row_stride, d.classes); if (rc != PXE_OK) return rc; }
-    const RowSpan x = group_span(d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes);
-    const RowSpan dx = group_span(d.dx, size, d.rows, inner, p.dx_outer_stride, p.dx_row_stride, d.classes);
-    PXE_REQUIRE(d.dx == d.x ? p.row_stride == p.dx_row_stride && p.outer_stride == p.dx_outer_stride : !rows_conflict(dx, x),
+    const Cover x = cover(d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes);
+    const Cover dx = cover(d.dx, size, d.rows, inner, p.dx_outer_stride, p.dx_row_stride, d.classes);
+    PXE_REQUIRE(d.dx == d.x ? p.row_stride == p.dx_row_stride && p.outer_stride == p.dx_outer_stride : !conflict(dx, x),
                 "log_probs_backward: dx partially overlaps x");
     const struct { const void* ptr; long long bytes; } ins[] = {{d.stats, d.rows * 12}, {d.dlogp, d.rows * 4}, {d.dentropy, d.rows * 4},
                                                                 {d.target, d.rows * (d.target_is_int64 ? 8 : 4)}};
     for (const auto& i : ins)
-        PXE_REQUIRE(!i.ptr || (i.ptr != d.dx && !rows_conflict({i.ptr, 1, 0, i.bytes}, dx)), "log_probs_backward: dx overlaps an input");
+        PXE_REQUIRE(!i.ptr || (i.ptr != d.dx && !conflict(RowSpan{i.ptr, 1, 0, i.bytes}, dx)), "log_probs_backward: dx overlaps an input");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d.type == PXE_F32) return launch_backward<float>(s, p);
     if (d.type == PXE_BF16) return launch_backward<bf16>(s, p);

@@ -926,7 +926,12 @@ extern "C" int pxe_rms_norm(pxe_stream_t stream, const pxe_rms_norm_desc* dp)
     PXE_REQUIRE(!d.weight || widest(d.weight, 0) >= wsize, "rms_norm: weight is not aligned to its elements");
     int vec = vec_for(access, C, size);
     if (d.weight && widest(d.weight, 0) < std::min(16, vec * wsize)) vec = 1;
-    const RowSpan stats{d.rstd, 1, 0, d.rows * 4}, scales{d.scale, 1, 0, d.rows * p.groups * 4};
+    const RowSpan stats{d.rstd, 1, 0, d.rows * 4}, scales{d.q ? d.scale : nullptr, 1, 0, d.rows * p.groups * 4}, weights{d.weight, 1, 0, (long long)C * wsize};
+    PXE_REQUIRE(((uintptr_t)d.rstd | (uintptr_t)scales.p) % 4 == 0, "rms_norm: rstd or scale is not aligned to its elements");
+    PXE_REQUIRE(!rows_conflict(stats, scales) && !(scales.p && scales.p == d.rstd) && !rows_conflict(stats, weights) && !rows_conflict(scales, weights) &&
+                !(d.weight && (d.weight == d.rstd || d.weight == scales.p)), "rms_norm: rstd, scale and weight overlap");
+    for (int i = 2; i < 5; ++i)
+        PXE_REQUIRE(!rows_conflict(span[i], weights) && !(d.weight && tensors[i].ptr == d.weight), "rms_norm: %s overlaps the weight", tensors[i].name);
     for (int i = 0; i < 5; ++i)
         PXE_REQUIRE(!(tensors[i].ptr && (tensors[i].ptr == d.rstd || (d.q && tensors[i].ptr == d.scale))) && !rows_conflict(span[i], stats) &&
                     !(d.q && rows_conflict(span[i], scales)), "rms_norm: rstd or scale overlaps %s", tensors[i].name);
@@ -986,6 +991,10 @@ extern "C" int pxe_rms_norm_backward(pxe_stream_t stream, const pxe_rms_norm_bac
     for (int i = 0; i < 3; ++i) PXE_REQUIRE(!rows_conflict(span[3], span[i]), "rms_norm_backward: dx partially overlaps %s", tensors[i].name);
     const int wsize = p.weight_f32 ? 4 : size;
     PXE_REQUIRE(!d.weight || widest(d.weight, 0) >= wsize, "rms_norm_backward: weight is not aligned to its elements");
+    PXE_REQUIRE((uintptr_t)d.rstd % 4 == 0, "rms_norm_backward: rstd is not aligned to its elements");
+    const RowSpan rstd{d.rstd, 1, 0, d.rows * 4}, weights{d.weight, 1, 0, (long long)C * wsize};
+    PXE_REQUIRE(!rows_conflict(span[3], rstd) && !rows_conflict(span[3], weights) && d.dx != (const void*)d.rstd && d.dx != d.weight,
+                "rms_norm_backward: dx overlaps rstd or the weight");
     const size_t need = d.dweight ? pxe_rms_norm_backward_workspace_bytes(d.rows, C) : 0;
     if (d.dweight) {
         PXE_REQUIRE(d.workspace && aligned16(d.workspace), "rms_norm_backward: dweight needs a 16-byte aligned workspace");
@@ -995,6 +1004,8 @@ extern "C" int pxe_rms_norm_backward(pxe_stream_t stream, const pxe_rms_norm_bac
             PXE_REQUIRE(!rows_conflict(ws, span[i]) && !rows_conflict(dw, span[i]) && d.workspace != tensors[i].ptr && d.dweight != tensors[i].ptr,
                         "rms_norm_backward: the workspace or dweight overlaps %s", tensors[i].name);
         PXE_REQUIRE(!rows_conflict(ws, dw) && d.workspace != (void*)d.dweight, "rms_norm_backward: the workspace overlaps dweight");
+        PXE_REQUIRE(!rows_conflict(ws, rstd) && !rows_conflict(dw, rstd) && !rows_conflict(ws, weights) && !rows_conflict(dw, weights) &&
+                    (const void*)d.dweight != d.weight && d.dweight != d.rstd, "rms_norm_backward: the workspace or dweight overlaps rstd or the weight");
     }
     p.partial = d.dweight ? static_cast<float*>(d.workspace) : nullptr;
     int vec = vec_for(access, C, size);

@@ -825,10 +825,12 @@ def softmax_cross_entropy(pred: torch.Tensor, truth: torch.Tensor):
 
 
 # ------------------------------------------------------------------------------ row operators in 32- and 16-bit types
-# A call on a token's row is as long as its marshalling, so these read each property of a tensor once and fill their
-# descriptors in one go.
+# A call on a token's row is as long as its marshalling: what holds is checked in line, a property at a time, and the
+# functions below that word a refusal are called only where something does not.
 _DTYPE = {torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16}
 _raw_stream = torch._C._cuda_getCurrentRawStream          # of a device's index; what current_stream(...).cuda_stream reads
+_current_device = torch._C._cuda_getDevice
+_f32 = torch.float32
 
 
 def _new(shape, dtype, device) -> torch.Tensor:
@@ -919,30 +921,49 @@ def _norm_weight(weight: Optional[torch.Tensor], channels: int, dtype, dev: int)
 
 
 def _rms_norm(x, weight, residual, eps, out, residual_out, e4m3, group):
-    dev = _rows_device(x, "x")
-    channels, dtype, shape = _channels(x, "x"), x.dtype, x.shape
-    wp, wtype = _norm_weight(weight, channels, dtype, dev)
-    rows = x.numel() // channels
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    kind = _DTYPE.get(dtype)
+    if kind is None or dev < 0 or dev != _current_device():
+        _rows_device(x, "x")
+    channels = shape[-1] if shape else 0
+    if not channels:
+        _channels(x, "x")
+    wp, wtype = None, capi.F32
+    if weight is not None:
+        if weight.dtype is _f32 and weight.dim() == 1 and weight.numel() == channels and weight.get_device() == dev and weight.is_contiguous():
+            wp = weight.data_ptr()
+        else:
+            wp, wtype = _norm_weight(weight, channels, dtype, dev)
     h, rp, rs, hp, hs = x, None, 0, None, 0
     if residual is not None:
-        _like(residual, shape, dtype, dev, "residual")
-        rp, rs = residual.data_ptr(), _row_stride(residual, "residual")
-        h = torch.empty_like(x) if residual_out is None else _like(residual_out, shape, dtype, dev, "residual_out")
-        hp, hs = h.data_ptr(), _row_stride(h, "residual_out")
+        if residual.shape != shape or residual.dtype is not dtype or residual.get_device() != dev:
+            _like(residual, shape, dtype, dev, "residual")
+        rp, rs = residual.data_ptr(), channels if residual.is_contiguous() else _row_stride(residual, "residual")
+        if residual_out is None:
+            h, hs = torch.empty_like(x, memory_format=torch.contiguous_format), channels
+        else:
+            h, hs = _like(residual_out, shape, dtype, dev, "residual_out"), _row_stride(residual_out, "residual_out")
+        hp = h.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    rstd = _new(shape[:-1], torch.float32, x.device)
-    kind = torch.float8_e4m3fn if e4m3 else dtype
-    y = torch.empty_like(x, dtype=kind) if out is None else _like(out, shape, kind, dev, "out")
-    yp, ys, scale, sp = y.data_ptr(), _row_stride(y, "out"), None, None
+    device, lead = x.device, shape[:-1]
+    rstd = _new(lead, _f32, device)
+    y_kind = torch.float8_e4m3fn if e4m3 else dtype
+    if out is None:
+        y, ys = torch.empty_like(x, dtype=y_kind, memory_format=torch.contiguous_format), channels
+    else:
+        y, ys = _like(out, shape, y_kind, dev, "out"), _row_stride(out, "out")
+    yp, qp, scale, sp, qs = y.data_ptr(), None, None, None, 0
     if e4m3:
-        scale = _new(shape[:-1] + (-(-channels // group) if group else 1,), torch.float32, x.device)
-        sp = scale.data_ptr()
+        scale = _new(lead + (-(-channels // group) if group else 1,), _f32, device)
+        sp, qp, qs, yp, ys = scale.data_ptr(), yp, ys, None, 0
+    rows = rstd.numel()
     if rows:
-        d = capi.RmsNormDesc(x.data_ptr(), rp, wp, hp, None if e4m3 else yp, yp if e4m3 else None, sp, rstd.data_ptr(),
-                             _row_stride(x, "x"), rs, hs, 0 if e4m3 else ys, ys if e4m3 else 0, rows, channels, _DTYPE[dtype], wtype,
-                             group, eps)
-        capi.check(capi.lib().pxe_rms_norm(_raw_stream(dev), C.byref(d)))
+        d = capi.RmsNormDesc(x.data_ptr(), rp, wp, hp, yp, qp, sp, rstd.data_ptr(), channels if x.is_contiguous() else _row_stride(x, "x"),
+                             rs, hs, ys, qs, rows, channels, kind, wtype, group, eps)
+        rc = capi.lib().pxe_rms_norm(_raw_stream(dev), C.byref(d))
+        if rc:
+            capi.check(rc)
     return y, scale, h, rstd
 
 
@@ -975,30 +996,41 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.
     alike; ``dresidual`` is the gradient that reaches ``h`` past the norm.  ``dweight`` (float32, ``None`` without a
     weight) is added to when given, as :func:`batchnorm_backward` does, and made otherwise.  ``dx`` may be ``dy``,
     ``h`` or ``dresidual``."""
-    dev = _rows_device(dy, "dy")
-    channels, dtype, shape = _channels(dy, "dy"), dy.dtype, dy.shape
+    shape, dtype, dev = dy.shape, dy.dtype, dy.get_device()
+    kind = _DTYPE.get(dtype)
+    if kind is None or dev < 0 or dev != _current_device():
+        _rows_device(dy, "dy")
+    channels = shape[-1] if shape else 0
+    if not channels:
+        _channels(dy, "dy")
     rows = dy.numel() // channels
-    _like(h, shape, dtype, dev, "h")
+    if h.shape != shape or h.dtype is not dtype or h.get_device() != dev:
+        _like(h, shape, dtype, dev, "h")
     wp, wtype = _norm_weight(weight, channels, dtype, dev)
     rp, rs = None, 0
     if dresidual is not None:
         _like(dresidual, shape, dtype, dev, "dresidual")
         rp, rs = dresidual.data_ptr(), _row_stride(dresidual, "dresidual")
-    dx = torch.empty_like(dy) if dx is None else _like(dx, shape, dtype, dev, "dx")
+    if dx is None:
+        dx, dxs = torch.empty_like(dy, memory_format=torch.contiguous_format), channels
+    else:
+        dxs = _row_stride(_like(dx, shape, dtype, dev, "dx"), "dx")
     accumulate, ws, wsp, nbytes, dwp = 0, None, None, 0, None
+    lib = capi.lib()
     if dweight is not None:
         dwp, accumulate = _dense_f32(dweight, channels, dev, "dweight"), 1
     elif weight is not None:
-        dweight = _new((channels,), torch.float32, dy.device)
+        dweight = _new((channels,), _f32, dy.device)
         dwp = dweight.data_ptr()
     if dwp is not None:
-        nbytes = capi.lib().pxe_rms_norm_backward_workspace_bytes(rows, channels)
+        nbytes = lib.pxe_rms_norm_backward_workspace_bytes(rows, channels)
         ws = _new((nbytes,), torch.uint8, dy.device)
         wsp = ws.data_ptr()
     d = capi.RmsNormBackwardDesc(dy.data_ptr(), h.data_ptr(), rp, wp, _dense_f32(rstd, rows, dev, "rstd"), dx.data_ptr(), dwp,
-                                 _row_stride(dy, "dy"), _row_stride(h, "h"), rs, _row_stride(dx, "dx"), rows, channels, _DTYPE[dtype],
-                                 wtype, accumulate, wsp, nbytes)
-    capi.check(capi.lib().pxe_rms_norm_backward(_raw_stream(dev), C.byref(d)))
+                                 _row_stride(dy, "dy"), _row_stride(h, "h"), rs, dxs, rows, channels, kind, wtype, accumulate, wsp, nbytes)
+    rc = lib.pxe_rms_norm_backward(_raw_stream(dev), C.byref(d))
+    if rc:
+        capi.check(rc)
     return dx, dweight
 
 
@@ -1034,26 +1066,32 @@ def log_probs(x: torch.Tensor, target: Optional[torch.Tensor] = None, *, top: in
     """Log probabilities of given classes, the entropy and the ``top`` (up to 32) most likely classes of every row of
     ``x`` [..., classes] (float32, bfloat16 or float16; a slice such as ``x[:, :-1]`` is read where it lies).  A negative
     ``target`` marks a row that is not used: zeros, and -1 for its alternatives.  Ties go to the lower class."""
-    dev = _rows_device(x, "x")
-    classes, shape = _channels(x, "x", "classes"), x.shape[:-1]
-    rows = x.numel() // classes
-    if not 0 <= top <= min(32, classes):
+    whole, dtype, dev = x.shape, x.dtype, x.get_device()
+    kind = _DTYPE.get(dtype)
+    if kind is None or dev < 0 or dev != _current_device():
+        _rows_device(x, "x")
+    classes = whole[-1] if whole else 0
+    if not classes:
+        _channels(x, "x", "classes")
+    if not 0 <= top <= 32 or top > classes:
         raise ValueError(f"top must lie in 0..{min(32, classes)}, got {top}")
-    f32 = torch.float32
+    device, shape = x.device, whole[:-1]
     logp = top_logp = top_index = tp = lp = vp = ip = None
     is64 = 0
     if target is not None:
         tp, is64 = _target(target, shape, dev)
-        logp = _new(shape, f32, x.device)
+        logp = _new(shape, _f32, device)
         lp = logp.data_ptr()
-    entropy, stats = _new(shape, f32, x.device), _new(shape + (3,), f32, x.device)
+    entropy, stats = _new(shape, _f32, device), _new(shape + (3,), _f32, device)
     if top:
-        top_logp, top_index = _new(shape + (top,), f32, x.device), _new(shape + (top,), torch.int32, x.device)
+        top_logp, top_index = _new(shape + (top,), _f32, device), _new(shape + (top,), torch.int32, device)
         vp, ip = top_logp.data_ptr(), top_index.data_ptr()
-    inner, outer, stride = _grouped_rows(x, "x")
-    d = capi.LogProbsDesc(x.data_ptr(), tp, lp, entropy.data_ptr(), stats.data_ptr(), vp, ip, rows, inner, outer, stride, classes,
-                          _DTYPE[x.dtype], is64, top, temperature)
-    capi.check(capi.lib().pxe_log_probs(_raw_stream(dev), C.byref(d)))
+    inner, outer, stride = (0, 0, classes) if x.is_contiguous() else _grouped_rows(x, "x")
+    d = capi.LogProbsDesc(x.data_ptr(), tp, lp, entropy.data_ptr(), stats.data_ptr(), vp, ip, entropy.numel(), inner, outer, stride, classes,
+                          kind, is64, top, temperature)
+    rc = capi.lib().pxe_log_probs(_raw_stream(dev), C.byref(d))
+    if rc:
+        capi.check(rc)
     return LogProbs(logp, entropy, top_logp, top_index, stats)
 
 
@@ -1063,24 +1101,32 @@ def log_probs_backward(x: torch.Tensor, target: Optional[torch.Tensor], stats: t
     """Gradient of :func:`log_probs` with respect to ``x``, from the gradients of ``logp`` and of ``entropy`` (float32, one
     for each row; either may be missing).  ``stats`` and ``temperature`` are the forward call's.  ``dx`` may be ``x``;
     without it the gradient gets x's own strides."""
-    dev = _rows_device(x, "x")
-    classes, shape = _channels(x, "x", "classes"), x.shape
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    kind = _DTYPE.get(dtype)
+    if kind is None or dev < 0 or dev != _current_device():
+        _rows_device(x, "x")
+    classes = shape[-1] if shape else 0
+    if not classes:
+        _channels(x, "x", "classes")
     rows = x.numel() // classes
     if dlogp is None and dentropy is None:
         raise ValueError("neither dlogp nor dentropy")
     if dlogp is not None and target is None:
         raise ValueError("dlogp without target")
     tp, is64 = _target(target, shape[:-1], dev) if target is not None else (None, 0)
-    inner, outer, stride = _grouped_rows(x, "x")
     if dx is None:
-        dx = torch.empty_strided(shape, x.stride(), device=x.device, dtype=x.dtype)
+        dx = torch.empty_strided(shape, x.stride(), device=x.device, dtype=dtype)
+        inner, outer, stride = (0, 0, classes) if x.is_contiguous() else _grouped_rows(x, "x")
         dx_outer, dx_stride = outer, stride
     else:
-        _, dx_outer, dx_stride = _grouped_rows(_like(dx, shape, x.dtype, dev, "dx"), "dx")
+        inner, outer, stride = _grouped_rows(x, "x")
+        _, dx_outer, dx_stride = _grouped_rows(_like(dx, shape, dtype, dev, "dx"), "dx")
     d = capi.LogProbsBackwardDesc(x.data_ptr(), tp, _dense_f32(stats, 3 * rows, dev, "stats"), _dense_f32(dlogp, rows, dev, "dlogp"),
                                   _dense_f32(dentropy, rows, dev, "dentropy"), dx.data_ptr(), rows, inner, outer, stride, dx_outer,
-                                  dx_stride, classes, _DTYPE[x.dtype], is64, temperature)
-    capi.check(capi.lib().pxe_log_probs_backward(_raw_stream(dev), C.byref(d)))
+                                  dx_stride, classes, kind, is64, temperature)
+    rc = capi.lib().pxe_log_probs_backward(_raw_stream(dev), C.byref(d))
+    if rc:
+        capi.check(rc)
     return dx
 
 
@@ -1100,11 +1146,13 @@ class AdamW:
         self.params = list(params)
         self.state_bits = state_bits
         self._dtype, self._device = torch.float32, None
+        dev = -1
+        if self.params:
+            dev = _rows_device(self.params[0], "params[0]")
+            self._dtype, self._device = self.params[0].dtype, self.params[0].device
         for i, p in enumerate(self.params):
-            _rows_device(p, f"params[{i}]")
-            if i == 0:
-                self._dtype, self._device = p.dtype, p.device
-            if p.dtype != self._dtype:
+            if p.dtype is not self._dtype or p.get_device() != dev:
+                _rows_device(p, f"params[{i}]")
                 raise TypeError(f"params[{i}] is {p.dtype}, the others {self._dtype}: one plan for each type")
             if not p.is_contiguous():
                 raise ValueError(f"params[{i}] must be contiguous")
@@ -1128,19 +1176,18 @@ class AdamW:
                 for w, p in zip(self.master, self.params):
                     w.copy_(p.detach().reshape(-1))
         count = len(self.params)
-        self._table = (capi.AdamwTensor * max(count, 1))()
         self._ptrs = [p.data_ptr() for p in self.params]
-        for i, row in enumerate(self._table[:count]):
-            row.param, row.n = self._ptrs[i], self._sizes[i]
-            row.m, row.v = self.m[i].data_ptr(), self.v[i].data_ptr()
-            if small:
-                row.m_scale, row.v_scale = self.m_scale[i].data_ptr(), self.v_scale[i].data_ptr()
-            if self.master is not None:
-                row.master = self.master[i].data_ptr()
-        # the addresses of the gradients, as a column of the table
-        self._grads = np.frombuffer(self._table, dtype=np.uint64).reshape(-1, C.sizeof(capi.AdamwTensor) // 8)[:count, capi.AdamwTensor.grad.offset // 8]
+        # the table the call reads, a pxe_adamw_tensor a row; the gradients' addresses change from step to step
+        self._table = np.zeros((max(count, 1), C.sizeof(capi.AdamwTensor) // 8), dtype=np.uint64)
+        column = lambda name: self._table[:count, getattr(capi.AdamwTensor, name).offset // 8]  # noqa: E731
+        column("param")[:] = self._ptrs
+        column("n")[:] = self._sizes
+        for name, tensors in (("m", self.m), ("v", self.v), ("m_scale", self.m_scale), ("v_scale", self.v_scale), ("master", self.master)):
+            if tensors is not None:
+                column(name)[:] = [t.data_ptr() for t in tensors]
+        self._grads = column("grad")
         d = self._desc = capi.AdamwDesc()
-        d.tensors, d.count, d.state_bits, d.param_type = C.addressof(self._table), count, state_bits, _DTYPE[self._dtype]
+        d.tensors, d.count, d.state_bits, d.param_type = self._table.ctypes.data, count, state_bits, _DTYPE[self._dtype]
 
     def _state(self, given, sizes, dtype, name):
         if given is None:                    # one buffer, every tensor on a 256-byte boundary
@@ -1153,10 +1200,10 @@ class AdamW:
         given = list(given)
         if len(given) != len(sizes):
             raise ValueError(f"{name} has {len(given)} tensors for {len(sizes)} parameters")
+        dev = self._device.index if sizes else -1
         for i, (t, n) in enumerate(zip(given, sizes)):
-            if not t.is_cuda or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
-                raise ValueError(f"{name}[{i}] must be a contiguous {dtype} CUDA tensor of {n} elements")
-            _check_device(t.device.index, f"{name}[{i}]")
+            if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+                raise ValueError(f"{name}[{i}] must be a contiguous {dtype} tensor of {n} elements on {self._device}")
         return given
 
     def _scalar(self, t, dtype, name):

@@ -457,6 +457,14 @@ def test_log_probs_slices_and_padding(cuda):
     buf = torch.full((3, 8, 107), 7.0, device="cuda", dtype=torch.bfloat16)                        # another distance from a boundary
     ops.log_probs_backward(keep[:, :-1], target[:, 1:].contiguous(), part.stats, d, dx=buf[..., 3:104])
     assert torch.equal(buf[..., 3:104], want) and bool((buf[..., :3] == 7).all()) and bool((buf[..., 104:] == 7).all())
+    both = torch.full((3, 9, 202), 7.0, device="cuda", dtype=torch.bfloat16)                       # columns of one buffer, and rows of one
+    both[..., :101] = keep
+    ops.log_probs_backward(both[:, :-1, :101], target[:, 1:].contiguous(), part.stats, d, dx=both[:, :-1, 101:])
+    assert torch.equal(both[:, :-1, 101:], want) and torch.equal(both[..., :101], keep) and bool((both[:, -1, 101:] == 7).all())
+    long = torch.zeros((3, 16, 101), device="cuda", dtype=torch.bfloat16)
+    long[:, :8] = keep[:, :-1]
+    ops.log_probs_backward(long[:, :8], target[:, 1:].contiguous(), part.stats, d, dx=long[:, 8:])
+    assert torch.equal(long[:, 8:], want)
     e = ops.log_probs(torch.empty(0, 7, device="cuda"), torch.empty(0, device="cuda", dtype=torch.int64), top=2)
     assert e.logp.shape == (0,) and e.top_index.shape == (0, 2)
     r = ops.log_probs(rand(36, (3, 50)), torch.tensor([1, 50, 1 << 40], device="cuda"))             # classes that are not there
@@ -800,3 +808,91 @@ def test_two_streams_at_once(cuda):
         torch.cuda.synchronize()
         for (dx, dw), (_, dx0, dw0) in zip(got, want):
             assert torch.equal(dx, dx0) and torch.equal(dw, dw0)
+
+
+def test_rows_beyond_32_bits(cuda):
+    """Rows more than 2^30 elements apart (offsets past 2^31), and a parameter of more than 2^31 elements: what lies there is
+    what the same rows and blocks give on their own."""
+    big = torch.zeros((1 << 31) + 8192, device="cuda", dtype=torch.bfloat16)
+    stride = (1 << 30) + 8
+    x, y = big.as_strided((3, 1000), (stride, 1)), big.as_strided((3, 1000), (stride, 1), 2048)
+    x.copy_(rand(500, (3, 1000), torch.bfloat16))
+    dense = x.contiguous()
+    w, target = rand(501, (1000,)), torch.tensor([5, 999, 0], device="cuda")
+    want, _, rstd = ops.rms_norm(dense, w)
+    ops.rms_norm(x, w, out=y)
+    assert torch.equal(y, want)
+    ops.rms_norm_backward(x, x, w, rstd, dx=y)
+    assert torch.equal(y, ops.rms_norm_backward(dense, dense, w, rstd)[0])
+    far, near = ops.log_probs(x, target, top=3), ops.log_probs(dense, target, top=3)
+    assert all(torch.equal(a, b) for a, b in zip(far, near))
+    d = rand(502, (3,))
+    ops.log_probs_backward(x, target, far.stats, d, dx=y)
+    assert torch.equal(y, ops.log_probs_backward(dense, target, near.stats, d))
+    del x, y
+    n = big.numel() - 5                                   # the last block is short
+    param, grad = big[:n], torch.full((n,), 0.5, device="cuda", dtype=torch.bfloat16)
+    tail = slice(n // 256 * 256 - 1024, n)
+    param[tail] = rand(503, (n - tail.start,), torch.bfloat16)
+    grad[tail] = rand(504, (n - tail.start,), torch.bfloat16)
+    small = [param[tail].clone()]
+    plan, alone = ops.AdamW([param], state_bits=8), ops.AdamW(small, state_bits=8)
+    plan.step([grad], rate=1e-2, t=1)
+    alone.step([grad[tail].clone()], rate=1e-2, t=1)
+    assert torch.equal(param[tail], small[0]) and torch.equal(plan.m[0][tail].view(torch.uint8), alone.m[0].view(torch.uint8))
+    assert torch.equal(plan.v_scale[0][-5:], alone.v_scale[0]) and bool((big[n:] == 0).all())
+    assert bool((param[4000:9000] == param[4000]).all()) and float(param[4000]) != 0            # (zeros before the step)
+
+
+def test_many_rows_of_few_classes(cuda):
+    x = rand(510, (70001, 3), torch.float16)
+    target = torch.randint(-1, 3, (70001,), device="cuda", generator=gen(511))
+    r, _ = check_probs(x, target, top=2)
+    d = rand(512, (70001,))
+    dx = ops.log_probs_backward(x, target, r.stats, d)
+    p = torch.softmax(x.double(), 1)
+    hot = torch.nn.functional.one_hot(target.clamp(min=0), 3).double()
+    want = (target >= 0).double()[:, None] * d.double()[:, None] * (hot - p)
+    within(dx, want, 64 * U * d.abs().double()[:, None] + half_step(torch.float16, want))
+    y, _, rstd = ops.rms_norm(x)
+    f = x.double()
+    r64 = 1 / (f.square().mean(1) + 1e-6).sqrt()
+    within(rstd, r64, r64 * 8 * U)
+    within(y, f * r64[:, None], (f * r64[:, None]).abs() * 10 * U + half_step(torch.float16, f * r64[:, None]))
+
+
+def test_a_captured_training_step_equals_the_eager_one(cuda):
+    """Norm, log probabilities, both gradients and the step captured in one graph, with t on the device, replayed on new
+    inputs: the bits of the eager calls (the weight gradient's second launch included)."""
+    n, c, v = 700, 1024, 511
+    x, res, head = rand(520, (n, c), torch.bfloat16), rand(521, (n, c), torch.bfloat16), rand(522, (v, c), torch.bfloat16, 0.1)
+    target, dlogp = torch.randint(0, v, (n,), device="cuda", generator=gen(523)), rand(524, (n,))
+    t = torch.zeros(1, device="cuda", dtype=torch.int64)
+
+    def step(weight, plan):
+        y, h, rstd = ops.rms_norm(x, weight, residual=res)
+        logits = y @ head.t()
+        r = ops.log_probs(logits, target)
+        dlogits = ops.log_probs_backward(logits, target, r.stats, dlogp, dx=logits)
+        dx, dweight = ops.rms_norm_backward(dlogits @ head, h, weight, rstd, dresidual=h)
+        plan.step([dweight], rate=1e-3, t=t, weight_decay=0.01)
+        return r.logp, dx, dweight
+
+    a, b = rand(525, (c,)), rand(525, (c,))
+    pa, pb = ops.AdamW([a]), ops.AdamW([b])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = rand(526, (c,))
+        step(warm, ops.AdamW([warm]))                     # (t is 0 here and its result is not looked at)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = step(b, pb)
+    torch.cuda.current_stream().wait_stream(side)
+    for k in (1, 2, 3):
+        x.copy_(rand(530 + k, (n, c), torch.bfloat16))
+        t.fill_(k)
+        graph.replay()
+        for got, want in zip(held, step(a, pa)):
+            assert torch.equal(got, want)
+        assert torch.equal(a, b) and torch.equal(pa.m[0], pb.m[0]) and torch.equal(pa.v[0], pb.v[0])

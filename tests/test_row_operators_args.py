@@ -50,6 +50,9 @@ def test_rms_norm_refusals():
     refused(norm(y=None, q=A, scale=E), "q overlaps x")
     refused(norm(rstd=A + 32), "rstd or scale overlaps")
     refused(norm(y=None, q=D, scale=A), "rstd or scale overlaps")
+    refused(norm(y=None, q=D, scale=C_ + 4), "rstd, scale and weight overlap")
+    refused(norm(weight=B_, weight_type=capi.F32), "y overlaps the weight")
+    refused(norm(rstd=C_ + 2), "not aligned")
     assert norm(rows=0) == capi.PXE_OK and norm(rows=0, x=None, rstd=None) == capi.PXE_OK
 
 
@@ -75,9 +78,12 @@ def test_rms_norm_backward_refusals_and_workspace():
     refused(back(dweight=A + 4, workspace=F, workspace_bytes=1 << 20), "overlaps dy")
     refused(back(dweight=F + 64, workspace=F, workspace_bytes=1 << 20), "overlaps dweight")
     refused(back(channels=1 << 20), "at most", capi.PXE_ERR_UNSUPPORTED)
+    refused(back(dx=C_), "overlaps rstd")
+    refused(back(dweight=C_, workspace=F, workspace_bytes=1 << 20), "overlaps rstd")
+    refused(back(weight=E, weight_type=capi.F32, dweight=E, workspace=F, workspace_bytes=1 << 20), "overlaps rstd or the weight")
     assert back(rows=0, dy=None) == capi.PXE_OK
     need = L.pxe_rms_norm_backward_workspace_bytes
-    assert need(0, 64) == 0 and need(3, 64) == 3 * 64 * 4 and need(1 << 30, 1023) <= 1024 * 1023 * 4
+    assert need(0, 64) == 0 and need(3, 64) == 3 * 64 * 4 and need(1 << 30, 1023) == 1184 * 1023 * 4 and need(1 << 30, 16384) == 148 * 16384 * 4
 
 
 def probs(**kw):
@@ -112,6 +118,9 @@ def test_log_probs_refusals():
     refused(probs(inner=4, outer_stride=300), "outer stride")
     refused(probs(entropy=A + 400), "overlaps")
     refused(probs(entropy=B_), "overlaps")
+    refused(probs(entropy=B_ + 28), "overlaps an input")
+    refused(probs(entropy=C_ + 4), "two outputs overlap")
+    refused(probs(entropy=D + 2), "not aligned")
     assert probs(rows=0, x=None) == capi.PXE_OK
 
 
@@ -134,6 +143,8 @@ def test_log_probs_backward_refusals():
     refused(probs_back(dx=A + 4), "partially overlaps x")
     refused(probs_back(dx=A, dx_row_stride=200), "partially overlaps x")
     refused(probs_back(dx=C_), "overlaps an input")
+    refused(probs_back(dx=A + 4 * 150, row_stride=200, dx_row_stride=200), "partially overlaps x")        # columns 150..250 of rows of 200
+    refused(probs_back(dx=A + 4 * 950, inner=4, outer_stride=1500, dx_outer_stride=1500, row_stride=300, dx_row_stride=300), "partially overlaps x")
     refused(probs_back(dx_row_stride=50), "row stride")
     refused(probs_back(temperature=0.0), "temperature")
     assert probs_back(rows=0, x=None) == capi.PXE_OK
