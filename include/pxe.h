@@ -708,7 +708,7 @@ PXE_API int pxe_log_probs(pxe_stream_t stream, const pxe_log_probs_desc* desc);
 
 /* Its gradient with respect to x, from dlogp and dentropy (either may be NULL, and a NULL target has no dlogp):
  *   dx_j = (dlogp * ([j == target] - p_j) - dentropy * p_j * (log p_j + entropy)) / temperature.
- * Rows that are not used, and rows of -inf throughout, have a gradient of 0; a target >= classes gives NaN.
+ * Rows that are not used, and rows of -inf throughout, have a gradient of 0; with dlogp a target >= classes gives NaN.
  * dx: `type`, addressed like x with its own strides; dx may be x. */
 typedef struct pxe_log_probs_backward_desc {
     const void* x;

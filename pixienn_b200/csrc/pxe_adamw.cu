@@ -126,7 +126,7 @@ __device__ __forceinline__ void store(T* p, const float (&f)[N])
     }
 }
 
-// One unit of 256 elements of a warp: loaded first, so that the next one's loads are on their way while this one is worked on.
+// One unit of 256 elements of a warp: all its loads, then the work on them.
 template <typename P, typename G, bool SMALL, bool MASTER, int N>
 struct Unit {
     using S = std::conditional_t<SMALL, uint8_t, float>;
@@ -215,6 +215,9 @@ __device__ __forceinline__ void one_unit(const Entry& e, long long first, int la
     u.work(e, first, lane, step);
 }
 
+// 64 M elements: fp32 with states in 32 bits 272 us, 1.07 of the copy rate; fp32 with states in 8 bits 158 us (1.06); bf16
+// with a master copy and states in 8 bits 164 us (1.01), without the copy 123 us (0.85, 12 bytes an element and as many
+// instructions).
 // Blocks of an SM: four (64 registers a thread, nothing spilled), six for 16-bit parameters with states in 8 bits, whose
 // lanes have half the bytes under way (64 M bf16 parameters: 122 against 134 us, with a master copy 164 against 167; fp32
 // parameters with states in 8 bits 157 against 171 us at six).

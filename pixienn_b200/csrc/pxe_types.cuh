@@ -21,7 +21,6 @@ inline int dtype_bytes(int t) { return t == PXE_F32 ? 4 : 2; }
 
 // ---------------------------------------------------------------- N elements as one access
 template <int BYTES> struct RawOf;
-template <> struct RawOf<32> { struct alignas(32) type { uint32_t w[8]; }; };
 template <> struct RawOf<16> { using type = uint4; };
 template <> struct RawOf<8> { using type = uint2; };
 template <> struct RawOf<4> { using type = uint32_t; };

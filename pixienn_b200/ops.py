@@ -1138,7 +1138,8 @@ class AdamW:
     float32 scale for every 256 elements (``m_scale``, ``v_scale``).  ``master=True`` keeps float32 copies of 16-bit
     parameters and updates those.  All are lists, one tensor for each parameter; lists of an earlier state can be given
     instead (a loaded checkpoint) and are then updated in place.  The plan holds the parameters; one whose memory
-    has moved since is refused by :meth:`step`."""
+    has moved since is refused by :meth:`step`.  The state's tensors stay the ones it was made with: to load another
+    state later, copy into them or make a new plan."""
 
     def __init__(self, params: Sequence[torch.Tensor], *, state_bits: int = 32, m=None, v=None, m_scale=None, v_scale=None, master=None):
         if state_bits not in (32, 8):

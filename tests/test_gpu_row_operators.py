@@ -896,3 +896,64 @@ def test_a_captured_training_step_equals_the_eager_one(cuda):
         for got, want in zip(held, step(a, pa)):
             assert torch.equal(got, want)
         assert torch.equal(a, b) and torch.equal(pa.m[0], pb.m[0]) and torch.equal(pa.v[0], pb.v[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [1030, 2000, 2051, 4100, 8190, 16383])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (1, 1)])
+def test_log_probs_of_many_rows_of_middling_length(cuda, dtype, v, pad, shift):
+    """Rows enough to fill the card, which are read by fewer threads each: a thread of the fewest adds v / 128 terms (to each
+    of two halves), a lane of a warp up to 64; both are under the v / 64 + 40 of a row eight times as long."""
+    n, info = 1300, torch.finfo(dtype)
+    x = rand(52, (n, v), dtype, 2.0, pad, shift)
+    x[0] = -INF                                           # nothing left
+    x[1] = -INF
+    x[1, v - 1] = 0.5                                     # one left
+    x[2] = info.min
+    x[3, 5:] = info.min
+    x[4] = info.max
+    x[5] = 0.0                                            # ties throughout
+    x[6] = torch.arange(v, device="cuda").to(dtype) % 7
+    x[7, 100:] = -INF
+    x[8, : v // 2] = 6.0                                  # more ties than any list holds
+    x[n - 1] = torch.linspace(-300, 300, v, device="cuda").to(dtype)
+    x[20:40, ::2] = -INF
+    target = torch.randint(0, v, (n,), device="cuda", generator=gen(53))
+    target[0], target[1] = 0, v - 1
+    target[50:90] = -1
+    target[n - 2] = -100
+    target[91] = v
+    for top, temperature in ((0, 1.0), (1, 0.7), (32, 1.0)):
+        r = ops.log_probs(x, target, top=top, temperature=temperature)
+        (logp, h, top_logp, top_index), _ = probs64(x, target, temperature, top)
+        tol = lambda want: probs_tol(8 * v, h if want.dim() == 1 else h[:, None], torch.nan_to_num(want, nan=0.0, neginf=0.0))  # noqa: E731
+        within(r.entropy, h, tol(h))
+        within(r.logp, logp, tol(logp))
+        if top:
+            assert torch.equal(r.top_index, top_index)
+            within(r.top_logp, top_logp, tol(top_logp))
+    x[9, v // 2], x[10, 1] = NAN, INF
+    r = ops.log_probs(x[9:11], top=2)
+    many = ops.log_probs(x, target.clamp(0, v - 1), top=2)
+    for got in (r, many._replace(logp=None, entropy=many.entropy[9:11], top_logp=many.top_logp[9:11], top_index=many.top_index[9:11])):
+        assert bool(got.entropy.isnan().all()) and bool(got.top_logp.isnan().all()) and got.top_index[:, 0].tolist() == [v // 2, 1]
+    assert bool(many.logp[9:11].isnan().all()) and bool(many.entropy[11:].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [130, 1025, 2047, 4096, 4111, 9000])
+def test_log_probs_gradient_of_rows_in_parts(cuda, dtype, v):
+    """Rows of one part and of several, whole vectors and single elements (where dx lies otherwise than x)."""
+    n = 37
+    x = rand(54, (n, v), dtype, 2.0, 3, 1)
+    target = torch.randint(-1, v, (n,), device="cuda", generator=gen(55))
+    d = rand(56, (n,))
+    r = ops.log_probs(x, target)
+    (_, h, _, _), lp = probs64(x, target, 1.0, 0)
+    hot = torch.zeros_like(lp).scatter_(1, target.clamp(min=0)[:, None], 1.0)
+    g = d.double()[:, None] * (target >= 0).double()[:, None]
+    want, size = g * (hot - lp.exp()), g.abs() * (hot + lp.exp())
+    tol = size * U * ((v / 64 + 40) + 200)
+    for dx in (None, torch.empty(n, v, device="cuda", dtype=dtype), torch.empty(n, v + 5, device="cuda", dtype=dtype)[:, 2:v + 2]):
+        got = ops.log_probs_backward(x, target, r.stats, d, dx=dx)
+        within(got, want, tol + half_step(dtype, want.abs() + tol) + 1e-37)
