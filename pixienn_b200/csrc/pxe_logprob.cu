@@ -21,8 +21,8 @@
 // first; keys are unique, so that exactly k threads are left.
 //
 // Few rows leave most SMs idle, so a long row is then split over a cluster of up to eight blocks, which exchange their
-// sums and their alternatives through distributed shared memory; short rows take one warp each and stay in its registers,
-// many rows of middling length a small block each.
+// sums and their alternatives through distributed shared memory; short rows take a warp or eight lanes of one each and
+// stay in registers, many rows of middling length a small block each.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -64,7 +64,7 @@ struct ProbsBackParams {
 
 __device__ __forceinline__ long long row_offset(long long row, long long inner, long long outer_stride, long long row_stride)
 {
-    const long long o = inner > 0 ? row / inner : 0;
+    const unsigned o = (unsigned)row / (unsigned)inner;    // (rows are less than 2^31, and inner at most rows)
     return o * outer_stride + (row - o * inner) * row_stride;
 }
 
@@ -598,10 +598,71 @@ log_probs_kernel(const ProbsParams p)
     }
 }
 
+constexpr int kShortThreads = 128;
+// Rows of up to 8 * NB vectors, without alternatives: eight lanes each, the row in registers.  Joining a row's lanes and
+// writing its results costs more instructions than so short a row itself; four rows of a warp share them.  65536 x 80 fp32:
+// 7.7 us, by a warp for each row 18.6 (L2 holds the rows; 3.2 at the copy rate); 65536 x 256 bf16: 10.9 and 21.3.
+constexpr int kPackedLanes = 8;
+template <typename T, int NB>
+__global__ void __launch_bounds__(kShortThreads)
+log_probs_packed_kernel(const ProbsParams p)
+{
+    constexpr int VEC = RowView<T>::VEC, LANES = kPackedLanes, NS = (2 * (VEC - 1) + LANES - 1) / LANES;
+    const int lane = threadIdx.x % LANES;
+    const long long row = (long long)blockIdx.x * (kShortThreads / LANES) + threadIdx.x / LANES;
+    const long long read = min(row, p.rows - 1);           // lanes behind the last row take part in the shuffles, and write nothing
+    const RowView<T> r(static_cast<const T*>(p.x) + row_offset(read, p.inner, p.outer_stride, p.row_stride), p.classes);
+    Raw<T, VEC> raw[NB];
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+        if (lane + LANES * k < r.nvec) raw[k] = gldv<Raw<T, VEC>>(r.x + r.element(lane + LANES * k));
+    float x[NB][VEC], x1[NS], m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {                         // the single elements in front and behind
+        const int i = lane + LANES * k, one = i < r.head ? i : r.tail() + i - r.head;
+        x1[k] = one < p.classes ? to_f32<T>(gld(r.x + one)) : -INFINITY;
+        m = max_nan(m, x1[k]);
+    }
+    const long long target = p.target ? target_of(p.target, p.target64, read) : 0;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+        unpack<T, VEC>(raw[k], x[k]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            if (lane + LANES * k >= r.nvec) x[k][j] = -INFINITY;
+            m = max_nan(m, x[k][j]);
+        }
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (m == -INFINITY) m = 0.0f;
+    float s = 0.0f, u = 0.0f;
+    auto add = [&](float v) {
+        const float d = distance(v, m, p.c), e = exp2_fast(d);
+        s += e;
+        u = fmaf(e, d, u);
+    };
+#pragma unroll
+    for (int k = 0; k < NS; ++k) add(x1[k]);
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) add(x[k][j]);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
+    if (lane != 0 || row >= p.rows) return;
+    const float l2s = log2f(s);
+    if (target < 0) store_unused(p, row, 0);
+    else store_row<T>(p, row, target, r.x, {m, s, u / s, l2s}, l2s);
+}
+
 // Rows of up to 32 * NB vectors: a warp each, the row in registers.  The maximum is known before the sums are formed.
-// 16384 x 1024 bf16: 10.6 us (L2 holds them), 65536 x 80 fp32: 18.6 us, where a row is shorter than the instructions that join
-// its lanes and write its results.
-constexpr int kShortThreads = 128, kShortCandidates = 128;
+// 16384 x 1024 bf16: 10.6 us (L2 holds them); 65536 x 80 fp32 with 8 alternatives: 42 us, bound by the instructions that find
+// them.
+constexpr int kShortCandidates = 128;
 template <typename T, int NB, bool TOP>
 __global__ void __launch_bounds__(kShortThreads)
 log_probs_short_kernel(const ProbsParams p)
@@ -817,22 +878,24 @@ int launch_with(cudaStream_t s, const ProbsParams& p, unsigned grid)
 }
 
 template <typename T, int NB>
+int launch_packed(cudaStream_t s, const ProbsParams& p)
+{
+    constexpr int rows = kShortThreads / kPackedLanes;
+    log_probs_packed_kernel<T, NB><<<(unsigned)((p.rows + rows - 1) / rows), kShortThreads, 0, s>>>(p);
+    PXE_LAUNCH_OK("log_probs_packed_kernel");
+    return PXE_OK;
+}
+
+template <typename T, int NB, bool TOP>
 int launch_short(cudaStream_t s, const ProbsParams& p)
 {
-    const unsigned grid = (unsigned)((p.rows + 3) / 4);
-    if constexpr (sizeof(T) == 4 || NB < 8) {
-        if (p.top) {
-            log_probs_short_kernel<T, NB, true><<<grid, kShortThreads, 0, s>>>(p);
-            PXE_LAUNCH_OK("log_probs_short_kernel");
-            return PXE_OK;
-        }
-    }
-    log_probs_short_kernel<T, NB, false><<<grid, kShortThreads, 0, s>>>(p);
+    log_probs_short_kernel<T, NB, TOP><<<(unsigned)((p.rows + 3) / 4), kShortThreads, 0, s>>>(p);
     PXE_LAUNCH_OK("log_probs_short_kernel");
     return PXE_OK;
 }
 
-// A row to a warp, in its registers, up to 128 vectors; without alternatives and in 32 bits up to 256 (16384 x 2000 bf16:
+// A row to eight lanes up to 32 vectors without alternatives; to a warp, in its registers, up to 128 vectors, and without
+// alternatives or in 32 bits up to 256 (16384 x 2000 bf16:
 // 16 us, by blocks of 64 threads 24; its 8 alternatives take a warp 111 us and blocks of 128 threads 53).  Above, what a
 // row's joining costs wants few threads where many rows wait, and few rows want many: up to 2048 vectors and when blocks
 // of 256 threads could not hold all rows at once, 64 threads, or 128 that look for alternatives (16384 x 4000 bf16: 34 us
@@ -845,10 +908,19 @@ int launch_forward(cudaStream_t s, ProbsParams& p, const DeviceInfo& di)
 {
     const int vecs = p.classes / (16 / (int)sizeof(T));
     p.cluster = 1;
-    if (vecs <= 32) return launch_short<T, 1>(s, p);
-    if (vecs <= 64) return launch_short<T, 2>(s, p);
-    if (vecs <= 128) return launch_short<T, 4>(s, p);
-    if (vecs <= 256 && (sizeof(T) == 4 || p.top == 0)) return launch_short<T, 8>(s, p);
+    if (p.top) {
+        if (vecs <= 32) return launch_short<T, 1, true>(s, p);
+        if (vecs <= 64) return launch_short<T, 2, true>(s, p);
+        if (vecs <= 128) return launch_short<T, 4, true>(s, p);
+        if constexpr (sizeof(T) == 4) { if (vecs <= 256) return launch_short<T, 8, true>(s, p); }
+    } else {
+        if (vecs <= kPackedLanes) return launch_packed<T, 1>(s, p);
+        if (vecs <= 2 * kPackedLanes) return launch_packed<T, 2>(s, p);
+        if (vecs <= 4 * kPackedLanes) return launch_packed<T, 4>(s, p);
+        if (vecs <= 64) return launch_short<T, 2, false>(s, p);
+        if (vecs <= 128) return launch_short<T, 4, false>(s, p);
+        if (vecs <= 256) return launch_short<T, 8, false>(s, p);
+    }
     if (vecs <= 2048 && p.rows > (long long)di.sm_count * kBlocks)
         return p.top ? launch_with<T, 128, true, false>(s, p, (unsigned)p.rows) : launch_with<T, 64, false, false>(s, p, (unsigned)p.rows);
     while (vecs > 4096 && p.cluster < 8 && p.rows * p.cluster * 2 <= 2LL * di.sm_count && vecs >= p.cluster * 2 * 256 * kBatch) p.cluster *= 2;
@@ -857,8 +929,9 @@ int launch_forward(cudaStream_t s, ProbsParams& p, const DeviceInfo& di)
     return p.top ? launch_with<T, 256, true, false>(s, p, grid) : launch_with<T, 256, false, false>(s, p, grid);
 }
 
-// A warp for every 128 vectors of rows of up to 512, a block for every 1024 of longer ones (16384 x 4000 bf16: 51 us, by
-// blocks 57; 8192 x 8000: 50 by warps, 43 by blocks; 65536 x 80 fp32: 23 and 175).
+// Eight lanes for rows of up to 32 vectors, a warp for every 128 vectors of rows of up to 512, a block for every 1024 of
+// longer ones (65536 x 80 fp32: 7.5 us, by warps 23; 16384 x 4000 bf16: 51 by warps, 57 by blocks; 8192 x 8000: 50 by warps,
+// 43 by blocks).
 template <typename T, int TPR>
 int launch_backward(cudaStream_t s, ProbsBackParams& p, int vecs)
 {
@@ -874,6 +947,7 @@ template <typename T>
 int launch_backward(cudaStream_t s, ProbsBackParams& p)
 {
     const int vecs = p.classes / (16 / (int)sizeof(T));
+    if (vecs <= 32) return launch_backward<T, 8>(s, p, vecs);
     return vecs <= 512 ? launch_backward<T, 32>(s, p, vecs) : launch_backward<T, kBackThreads>(s, p, vecs);
 }
 

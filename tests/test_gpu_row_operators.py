@@ -957,3 +957,43 @@ def test_log_probs_gradient_of_rows_in_parts(cuda, dtype, v):
     for dx in (None, torch.empty(n, v, device="cuda", dtype=dtype), torch.empty(n, v + 5, device="cuda", dtype=dtype)[:, 2:v + 2]):
         got = ops.log_probs_backward(x, target, r.stats, d, dx=dx)
         within(got, want, tol + half_step(dtype, want.abs() + tol) + 1e-37)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v", [(1, 1), (15, 3), (16, 7), (17, 31), (1000, 32), (33, 40), (1001, 80), (50, 127), (19, 128), (65, 200), (31, 257), (15, 263)])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (1, 1), (5, 3)])
+def test_log_probs_of_short_rows(cuda, dtype, n, v, pad, shift):
+    """Rows that share a warp, with their gradient: masked ones, unused ones and a last warp that is not full."""
+    x = rand(57, (n, v), dtype, 2.0, pad, shift)
+    x[n // 2] = -INF
+    x[n // 3, 1:] = -INF
+    if n > 8:
+        x[2] = torch.finfo(dtype).min
+        x[3] = 0.0
+        x[7, v - 1] = -INF
+    target = torch.randint(0, v, (n,), device="cuda", generator=gen(58))
+    target[n // 2] = 0
+    check_probs(x, None, temperature=0.5)
+    check_probs(x, target.int())
+    target[n // 4::5] = -1
+    if n > 8:
+        target[6] = v
+    r, lp = check_probs(x, target, temperature=1.5)
+    assert torch.equal(r.stats[target < 0], torch.zeros_like(r.stats[target < 0]))
+    target = target.clamp(max=v - 1)
+    d = rand(59, (n,))
+    used = ((target >= 0) & (x != -INF).any(1)).double()[:, None]
+    p = torch.nan_to_num(lp, neginf=-1e9).exp()
+    hot = torch.zeros_like(p).scatter_(1, target.clamp(min=0)[:, None], 1.0)
+    size = used * d.double()[:, None].abs() * (hot + p) / 1.5
+    want = used * d.double()[:, None] * (hot - p) / 1.5
+    tol = size * U * ((v / 512 + 40) + 200)
+    within(ops.log_probs_backward(x, target, r.stats, d, temperature=1.5), want, tol + half_step(dtype, want.abs() + tol) + 1e-37)
+    if n > 8:
+        wide = x[6:n - n % 2].reshape(2, -1, v)[:, 1:]     # groups of rows, where they lie
+        a, b = ops.log_probs(wide), ops.log_probs(wide.contiguous())
+        within(a.entropy, b.entropy, 2 * probs_tol(v, torch.nan_to_num(b.entropy), torch.nan_to_num(b.entropy)))
+    if n > 20:
+        x[11, v // 2], x[12, 0] = NAN, INF
+        r = ops.log_probs(x, target.clamp(min=0))
+        assert bool(r.logp[11:13].isnan().all()) and bool(r.entropy[11:13].isnan().all()) and bool(r.entropy[13:].isfinite().all())
