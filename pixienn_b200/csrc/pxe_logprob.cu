@@ -62,9 +62,13 @@ struct ProbsBackParams {
     float c, inv_temperature;
 };
 
+// Where a row begins.  Rows are less than 2^31 and inner at most rows, so that 32 bits would do for the division; they are
+// used where short rows share a block (65536 x 80 fp32).  Where a block has one row the division counts for nothing, but
+// its result then stays in registers that the sums need (4095 x 50003 bf16: 77 us, 20 bytes spilled, against 71).
+template <typename INT>
 __device__ __forceinline__ long long row_offset(long long row, long long inner, long long outer_stride, long long row_stride)
 {
-    const unsigned o = (unsigned)row / (unsigned)inner;    // (rows are less than 2^31, and inner at most rows)
+    const long long o = (INT)row / (INT)inner;
     return o * outer_stride + (row - o * inner) * row_stride;
 }
 
@@ -508,7 +512,7 @@ log_probs_kernel(const ProbsParams p)
         if (rank == 0) store_unused(p, row, t);
         return;
     }
-    Slice<T> s{RowView<T>(static_cast<const T*>(p.x) + row_offset(row, p.inner, p.outer_stride, p.row_stride), p.classes), 0, 0, rank == 0, rank == ranks - 1};
+    Slice<T> s{RowView<T>(static_cast<const T*>(p.x) + row_offset<long long>(row, p.inner, p.outer_stride, p.row_stride), p.classes), 0, 0, rank == 0, rank == ranks - 1};
     const RowView<T>& r = s.r;
     const int per = (r.nvec + ranks - 1) / ranks;
     s.v0 = min(rank * per, r.nvec);
@@ -611,7 +615,7 @@ log_probs_packed_kernel(const ProbsParams p)
     const int lane = threadIdx.x % LANES;
     const long long row = (long long)blockIdx.x * (kShortThreads / LANES) + threadIdx.x / LANES;
     const long long read = min(row, p.rows - 1);           // lanes behind the last row take part in the shuffles, and write nothing
-    const RowView<T> r(static_cast<const T*>(p.x) + row_offset(read, p.inner, p.outer_stride, p.row_stride), p.classes);
+    const RowView<T> r(static_cast<const T*>(p.x) + row_offset<unsigned>(read, p.inner, p.outer_stride, p.row_stride), p.classes);
     Raw<T, VEC> raw[NB];
 #pragma unroll
     for (int k = 0; k < NB; ++k)
@@ -672,7 +676,7 @@ log_probs_short_kernel(const ProbsParams p)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long row = (long long)blockIdx.x * WARPS + warp;
     if (row >= p.rows) return;
-    const RowView<T> r(static_cast<const T*>(p.x) + row_offset(row, p.inner, p.outer_stride, p.row_stride), p.classes);
+    const RowView<T> r(static_cast<const T*>(p.x) + row_offset<unsigned>(row, p.inner, p.outer_stride, p.row_stride), p.classes);
     // what a lane takes of the row: NB vectors, and one of the single elements in front and behind (at most 2 * (VEC - 1))
     Raw<T, VEC> raw[NB];
 #pragma unroll
@@ -777,14 +781,15 @@ __global__ void __launch_bounds__(kBackThreads)
 log_probs_backward_kernel(const ProbsBackParams p)
 {
     constexpr int VEC = RowView<T>::VEC;
+    using Index = std::conditional_t<TPR == kBackThreads, long long, unsigned>;
     const int t = threadIdx.x % TPR;
     const unsigned part = blockIdx.x * (kBackThreads / TPR) + threadIdx.x / TPR;   // (at most 2^31 + 8)
     const unsigned behind = part / (unsigned)p.chunks;
     const int chunk = (int)(part - behind * (unsigned)p.chunks);
     const long long row = p.rows - 1 - behind;
     if (row < 0) return;
-    const T* x = static_cast<const T*>(p.x) + row_offset(row, p.inner, p.outer_stride, p.row_stride);
-    T* dx = static_cast<T*>(p.dx) + row_offset(row, p.inner, p.dx_outer_stride, p.dx_row_stride);
+    const T* x = static_cast<const T*>(p.x) + row_offset<Index>(row, p.inner, p.outer_stride, p.row_stride);
+    T* dx = static_cast<T*>(p.dx) + row_offset<Index>(row, p.inner, p.dx_outer_stride, p.dx_row_stride);
     const RowView<T> r(x, p.classes);
     const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
     const int first = chunk * TPR * kBatch + t;
