@@ -997,3 +997,23 @@ def test_log_probs_of_short_rows(cuda, dtype, n, v, pad, shift):
         x[11, v // 2], x[12, 0] = NAN, INF
         r = ops.log_probs(x, target.clamp(min=0))
         assert bool(r.logp[11:13].isnan().all()) and bool(r.entropy[11:13].isnan().all()) and bool(r.entropy[13:].isfinite().all())
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(cuda, monkeypatch):
+    """Launches go to the current device: with another one current, every call is refused before anything is launched."""
+    x, w = rand(60, (4, 64)), rand(61, (64,))
+    target = torch.zeros(4, dtype=torch.int64, device="cuda")
+    _, h, rstd = ops.rms_norm(x, w)
+    r = ops.log_probs(x, target)
+    plan = ops.AdamW([w])
+    torch.cuda.synchronize()
+    before = w.clone()
+    with monkeypatch.context() as m:
+        m.setattr(ops, "_current_device", lambda: 1)
+        m.setattr(torch.cuda, "current_device", lambda: 1)
+        for call in (lambda: ops.rms_norm(x, w), lambda: ops.rms_norm_e4m3(x, w), lambda: ops.rms_norm_backward(x, h, w, rstd),
+                     lambda: ops.log_probs(x, target), lambda: ops.log_probs_backward(x, target, r.stats, rstd),
+                     lambda: ops.AdamW([w]), lambda: plan.step([w.clone()], rate=1.0, t=1)):
+            with pytest.raises((ValueError, RuntimeError), match="device"):
+                call()
+    assert torch.equal(w, before)
