@@ -8,10 +8,13 @@
 // issue slots an element on an SM.  Each thread takes four 16-byte vectors at a time, finds their maximum (two elements
 // an instruction in 16 bits), rescales its sums only when the running maximum grows, and forms d = x * c - o with one
 // rounding from the origin o = fl(m * c), two elements an instruction (as S and U).  The origin's rounding is the same
-// shift for every element and is taken out of log2 S at the end.  Values of -inf are held at -2^100 (the lowest value
-// in fp16), so that a probability of 0 adds 0 * d = 0 to U.  A row whose maximum lies beyond +-1e30 (under half the lowest
-// value in fp16), such as one masked throughout with the type's lowest value, is read again with (x - m) * c, which
-// neither overflows nor loses the row; so is every row at temperatures above 72 or below 1e-7.
+// shift for every element, up to half a unit of o, and is taken out of log2 S at the end: at |m c| <= 2^24 it is at most
+// 1/2.  Beyond, 2^shift would leave the range of a float (at m = -1e10 and temperature 1 the shift is 440), so that
+// partial sums under a maximum of m c < -2^24 take the origin 0 instead, from which all they hold adds 0 (a mask's finite
+// value, until the thread or another one meets more), and a row whose own maximum lies beyond +-2^24 / c is read again
+// with (x - m) * c, which neither overflows nor loses the row.  So is every row at temperatures above 72 or below 1e-7, and
+// one in fp16 under half the lowest value: values of -inf are held at -2^100 (the lowest value in fp16), so that a
+// probability of 0 adds 0 * d = 0 to U, and count for nothing only from further away.
 //
 // The alternatives need no second pass over the row.  The k-th largest of the threads' own maxima is a lower bound of the
 // k-th largest value of all, and whatever reaches it lies with the threads whose maximum does: k of them, and those that
@@ -47,7 +50,7 @@ struct ProbsParams {
     int* top_index;
     long long rows, inner, outer_stride, row_stride;
     int classes, target64, top, cluster, careful;
-    float c, inv_temperature;
+    float c, inv_temperature, far;                         // far = kFar / c
 };
 
 struct ProbsBackParams {
@@ -88,9 +91,13 @@ __device__ __forceinline__ float distance(float x, float m, float c) { return ma
 struct Part {
     float m, s, u;
 };
-constexpr float kFar = 1e30f;
+constexpr float kFar = 16777216.0f;                        // of m * c: its rounding shifts the sums by half a unit, 2^(1/2) of them
 // (a product that is never contracted into what uses it: the origin's rounding has to be the same everywhere)
-__device__ __forceinline__ float origin_of(float m, float c) { return m < -kFar ? 0.0f : __fmul_rn(m, c); }
+__device__ __forceinline__ float origin_of(float m, float c)
+{
+    const float o = __fmul_rn(m, c);
+    return o < -kFar ? 0.0f : o;
+}
 
 __device__ __forceinline__ void rescale(float& s, float& u, float from, float to)
 {
@@ -108,17 +115,17 @@ __device__ __forceinline__ Part join(Part a, Part b, float c)
 }
 
 // 32-bit words of a vector: one float or two 16-bit elements each.  LOW, low: what -inf is held at; a row whose maximum is
-// under `lowest` is too near to that and read again.
+// under `lowest` is too near to that and read again (in 32 bits and bf16 such a row is beyond -2^24 / c already).
 template <typename T> struct Word;
 template <> struct Word<float> {
     static constexpr uint32_t LOW = 0xf1800000u, NONE = 0xff800000u;               // -2^100, -inf
-    static constexpr float low = -0x1p100f, lowest = -kFar;
+    static constexpr float low = -0x1p100f, lowest = -INFINITY;
     static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
     static __device__ __forceinline__ float largest(uint32_t a) { return __uint_as_float(a); }
 };
 template <> struct Word<bf16> {
     static constexpr uint32_t LOW = 0xf180f180u, NONE = 0xff80ff80u;               // -2^100, -inf
-    static constexpr float low = -0x1p100f, lowest = -kFar;
+    static constexpr float low = -0x1p100f, lowest = -INFINITY;
     static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b)
     {
         uint32_t r;
@@ -556,7 +563,7 @@ log_probs_kernel(const ProbsParams p)
     Part all = join_all(sum.part());
     const float m = all.m == -INFINITY ? 0.0f : all.m;
     float l2s;
-    if (m < Word<T>::lowest || (m > kFar && m < INFINITY) || p.careful) {     // the whole row again, from its maximum
+    if ((fabsf(m) > p.far && m < INFINITY) || m < Word<T>::lowest || p.careful) {                 // the whole row again, from its maximum
         Part again{0.0f, 0.0f, 0.0f};                  // (one origin for all: the sums add up)
         auto careful = [&](float x) {
             const float d = distance(x, m, p.c), e = exp2_fast(d);
@@ -1025,6 +1032,7 @@ extern "C" int pxe_log_probs(pxe_stream_t stream, const pxe_log_probs_desc* dp)
     DeviceInfo di;
     { const int rc = device_info(&di); if (rc != PXE_OK) return rc; }
     p.careful = !(p.c > 0.02f && p.c < 1e7f);              // what -inf is held at would count, or overflow
+    p.far = kFar / p.c;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d.type == PXE_F32) return launch_forward<float>(s, p, di);
     if (d.type == PXE_BF16) return launch_forward<bf16>(s, p, di);
