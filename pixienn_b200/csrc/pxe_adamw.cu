@@ -307,6 +307,8 @@ extern "C" int pxe_adamw_update(pxe_stream_t stream, const pxe_adamw_desc* dp)
     PXE_REQUIRE(d.beta1 >= 0.0f && d.beta1 < 1.0f && d.beta2 >= 0.0f && d.beta2 < 1.0f, "adamw_update: beta1 and beta2 lie in [0, 1)");
     PXE_REQUIRE(d.eps >= 0.0f, "adamw_update: eps is negative or NaN");
     PXE_REQUIRE(d.t_device || d.t >= 1, "adamw_update: step %lld (the first step is 1)", d.t);
+    PXE_REQUIRE(((uintptr_t)d.rate_device | (uintptr_t)d.grad_scale_device | (uintptr_t)d.skip_device) % 4 == 0 && (uintptr_t)d.t_device % 8 == 0,
+                "adamw_update: a device scalar is not aligned to its type");
     const bool small = d.state_bits == 8;
     const int psize = dtype_bytes(d.param_type), gsize = dtype_bytes(d.grad_type), ssize = small ? 1 : 4;
     bool master = false, first = true;

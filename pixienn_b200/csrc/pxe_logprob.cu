@@ -1020,6 +1020,7 @@ extern "C" int pxe_log_probs(pxe_stream_t stream, const pxe_log_probs_desc* dp)
     const Cover x = cover(d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes);
     const struct { const void* ptr; long long bytes; } outs[] = {{d.logp, d.rows * 4}, {d.entropy, d.rows * 4}, {d.stats, d.rows * 12},
                                                                  {d.top_logp, d.rows * d.top * 4}, {d.top_index, d.rows * d.top * 4}};
+    PXE_REQUIRE(reinterpret_cast<uintptr_t>(d.target) % (d.target_is_int64 ? 8 : 4) == 0, "log_probs: target is not aligned to its elements");
     const RowSpan target{d.target, 1, 0, d.rows * (d.target_is_int64 ? 8 : 4)};
     for (const auto& o : outs) {
         if (!o.ptr) continue;
@@ -1066,10 +1067,13 @@ extern "C" int pxe_log_probs_backward(pxe_stream_t stream, const pxe_log_probs_b
     const Cover dx = cover(d.dx, size, d.rows, inner, p.dx_outer_stride, p.dx_row_stride, d.classes);
     PXE_REQUIRE(d.dx == d.x ? p.row_stride == p.dx_row_stride && p.outer_stride == p.dx_outer_stride : !conflict(dx, x),
                 "log_probs_backward: dx partially overlaps x");
-    const struct { const void* ptr; long long bytes; } ins[] = {{d.stats, d.rows * 12}, {d.dlogp, d.rows * 4}, {d.dentropy, d.rows * 4},
-                                                                {d.target, d.rows * (d.target_is_int64 ? 8 : 4)}};
-    for (const auto& i : ins)
+    const int tsize = d.target_is_int64 ? 8 : 4;
+    const struct { const void* ptr; long long bytes; int align; } ins[] = {{d.stats, d.rows * 12, 4}, {d.dlogp, d.rows * 4, 4},
+                                                                           {d.dentropy, d.rows * 4, 4}, {d.target, d.rows * tsize, tsize}};
+    for (const auto& i : ins) {
+        PXE_REQUIRE(reinterpret_cast<uintptr_t>(i.ptr) % i.align == 0, "log_probs_backward: an input is not aligned to its elements");
         PXE_REQUIRE(!i.ptr || (i.ptr != d.dx && !conflict(RowSpan{i.ptr, 1, 0, i.bytes}, dx)), "log_probs_backward: dx overlaps an input");
+    }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d.type == PXE_F32) return launch_backward<float>(s, p);
     if (d.type == PXE_BF16) return launch_backward<bf16>(s, p);
