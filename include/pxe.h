@@ -735,8 +735,8 @@ PXE_API int pxe_log_probs_backward(pxe_stream_t stream, const pxe_log_probs_back
  * PXE_ADAMW_BLOCK elements (scale = max(largest / 448, 2^-126) of the new values; a v above zero keeps a code above
  * zero); arithmetic stays in fp32.  A gradient that is not finite spoils its element, and in 8 bits its block.
  * `tensors` is a HOST array that the call reads before it returns; entries with n == 0 are passed over.  Nothing may
- * overlap anything else: parameters, states and masters that do are refused.  The step is one launch for every
- * PXE_ADAMW_TENSORS_PER_LAUNCH tensors, with no workspace. */
+ * overlap anything else: parameters, states, masters and device scalars that do are refused.  The step is one launch for
+ * every PXE_ADAMW_TENSORS_PER_LAUNCH tensors, with no workspace. */
 #define PXE_ADAMW_BLOCK 256
 #define PXE_ADAMW_TENSORS_PER_LAUNCH 400
 typedef struct pxe_adamw_tensor {

@@ -336,6 +336,11 @@ extern "C" int pxe_adamw_update(pxe_stream_t stream, const pxe_adamw_desc* dp)
                 if (p[family]) ranges.push_back({(uintptr_t)p[family], (uintptr_t)p[family] + (uintptr_t)bytes[family], family != 1});
             }
         }
+        const struct { uintptr_t lo, bytes; } scalars[4] = {{(uintptr_t)d.rate_device, 4}, {(uintptr_t)d.t_device, 8},
+                                                         {(uintptr_t)d.grad_scale_device, 4}, {(uintptr_t)d.skip_device, 4}};
+        for (const auto& x : scalars)
+            for (const Range& r : ranges)
+                PXE_REQUIRE(!x.lo || !r.written || x.lo >= r.hi || x.lo + x.bytes <= r.lo, "adamw_update: a device scalar lies inside what the step writes");
         PXE_REQUIRE(!ranges_conflict(ranges), "adamw_update: tensors overlap (one listed twice, or a state, master or gradient inside another)");
     } catch (const std::exception& e) {
         return set_error(PXE_ERR_CUDA, "adamw_update: %s", e.what());

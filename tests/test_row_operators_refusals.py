@@ -1,6 +1,8 @@
 """More calls that the row operators refuse on the host, before anything touches a device (the addresses here are never
 dereferenced), and what they no longer refuse."""
-from test_row_operators_args import B_, C_, D, E, F, adamw, probs, probs_back, refused
+from pixienn_b200 import capi
+
+from test_row_operators_args import A, B_, C_, D, E, F, adamw, probs, probs_back, refused
 
 
 def test_log_probs_refuse_inputs_off_their_elements():
@@ -15,3 +17,13 @@ def test_log_probs_refuse_inputs_off_their_elements():
 def test_adamw_refuses_device_scalars_off_their_elements():
     for name, off in (("rate_device", 2), ("grad_scale_device", 1), ("skip_device", 2), ("t_device", 4)):
         refused(adamw([{}], **{name: E + off}), "not aligned")
+
+
+def test_adamw_refuses_device_scalars_inside_what_it_writes():
+    """A block would read the scalar while another writes it."""
+    for name in ("rate_device", "grad_scale_device", "skip_device", "t_device"):
+        for inside in (A, A + 3992, C_ + 8, D + 3992):
+            refused(adamw([{}], **{name: inside}), "device scalar")
+    refused(adamw([{}, {"param": E, "grad": B_ + 8000, "m": C_ + 8000, "v": F}], t_device=F + 3992), "device scalar")
+    refused(adamw([{"m_scale": E, "v_scale": F}], state_bits=8, rate_device=F + 12), "device scalar")
+    refused(adamw([{"master": E}], param_type=capi.BF16, grad_type=capi.BF16, skip_device=E), "device scalar")
