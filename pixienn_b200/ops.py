@@ -830,6 +830,7 @@ def softmax_cross_entropy(pred: torch.Tensor, truth: torch.Tensor):
 _DTYPE = {torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16}
 _raw_stream = torch._C._cuda_getCurrentRawStream          # of a device's index; what current_stream(...).cuda_stream reads
 _current_device = torch._C._cuda_getDevice
+_data_ptr = torch.Tensor.data_ptr
 _f32 = torch.float32
 
 
@@ -1137,9 +1138,9 @@ class AdamW:
     keeps ``m`` and ``v`` as float32; ``state_bits=8`` keeps ``m`` and the root of ``v`` as float8_e4m3fn codes with a
     float32 scale for every 256 elements (``m_scale``, ``v_scale``).  ``master=True`` keeps float32 copies of 16-bit
     parameters and updates those.  All are lists, one tensor for each parameter; lists of an earlier state can be given
-    instead (a loaded checkpoint) and are then updated in place.  The plan holds the parameters; one whose memory
-    has moved since is refused by :meth:`step`.  The state's tensors stay the ones it was made with: to load another
-    state later, copy into them or make a new plan."""
+    instead (a loaded checkpoint) and are then updated in place.  The plan holds the parameters and the state; a tensor
+    of either that was replaced, or whose memory has moved since, is refused by :meth:`step`.  To load another state
+    later, copy into the tensors or make a new plan."""
 
     def __init__(self, params: Sequence[torch.Tensor], *, state_bits: int = 32, m=None, v=None, m_scale=None, v_scale=None, master=None):
         if state_bits not in (32, 8):
@@ -1177,15 +1178,16 @@ class AdamW:
                 for w, p in zip(self.master, self.params):
                     w.copy_(p.detach().reshape(-1))
         count = len(self.params)
-        self._ptrs = [p.data_ptr() for p in self.params]
+        # what the table's addresses belong to, kept so that nothing else can take their place, and the addresses
+        self._held = [(name, list(tensors), list(map(_data_ptr, tensors))) for name, tensors in
+                      (("params", self.params), ("m", self.m), ("v", self.v), ("m_scale", self.m_scale), ("v_scale", self.v_scale),
+                       ("master", self.master)) if tensors is not None]
         # the table the call reads, a pxe_adamw_tensor a row; the gradients' addresses change from step to step
         self._table = np.zeros((max(count, 1), C.sizeof(capi.AdamwTensor) // 8), dtype=np.uint64)
         column = lambda name: self._table[:count, getattr(capi.AdamwTensor, name).offset // 8]  # noqa: E731
-        column("param")[:] = self._ptrs
         column("n")[:] = self._sizes
-        for name, tensors in (("m", self.m), ("v", self.v), ("m_scale", self.m_scale), ("v_scale", self.v_scale), ("master", self.master)):
-            if tensors is not None:
-                column(name)[:] = [t.data_ptr() for t in tensors]
+        for name, _, ptrs in self._held:
+            column("param" if name == "params" else name)[:] = ptrs
         self._grads = column("grad")
         d = self._desc = capi.AdamwDesc()
         d.tensors, d.count, d.state_bits, d.param_type = self._table.ctypes.data, count, state_bits, _DTYPE[self._dtype]
@@ -1219,8 +1221,7 @@ class AdamW:
         of one type (float32 or the parameters' own; any of the three types for float32 parameters).  ``t`` counts steps
         from 1.  ``rate``, ``grad_scale`` (float32) and ``t`` (int64) may be CUDA tensors of one element, which a captured
         step reads at every replay; ``skip``: a float32 one that, not 0, makes the step do nothing."""
-        params = self.params
-        count = len(params)
+        count = len(self._sizes)
         if len(grads) != count:
             raise ValueError(f"{len(grads)} gradients for {count} parameters")
         if count == 0:
@@ -1228,8 +1229,9 @@ class AdamW:
         dev = self._device.index
         if dev != torch.cuda.current_device():
             _check_device(dev, "params")
-        if [p.data_ptr() for p in params] != self._ptrs:
-            raise RuntimeError("a parameter's memory has moved since this plan was made; make a new one")
+        for name, _, ptrs in self._held:
+            if list(map(_data_ptr, getattr(self, name))) != ptrs:
+                raise RuntimeError(f"{name}: a tensor was replaced or its memory has moved since this plan was made; make a new one")
         kind = getattr(grads[0], "dtype", None)
         if kind not in _DTYPE:
             raise TypeError(f"gradients must be float32, bfloat16 or float16 tensors, got {kind}")

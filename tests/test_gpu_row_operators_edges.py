@@ -92,3 +92,37 @@ def test_log_probs_of_many_rows_with_finite_masks(cuda, dtype, v):
             m = min(len(rows), len(x) - k)
             within(got.entropy[k:k + m], few.entropy[:m], tol[:m])
             assert top == 0 or torch.equal(got.top_index[k:k + m], few.top_index[:m])
+
+
+# ------------------------------------------------------------------------------------------------ AdamW
+def test_adamw_refuses_a_state_that_was_replaced(cuda):
+    """The step writes where the plan's state was when it was made: another tensor in one of its lists, another list, or other
+    memory behind a tensor is refused; copying into the state is what loads another one."""
+    for bits in (32, 8):
+        params, grads = [rand(700, (300,), torch.bfloat16), rand(701, (70,), torch.bfloat16)], [rand(702, (300,), torch.bfloat16), rand(703, (70,), torch.bfloat16)]
+        plan = ops.AdamW(params, state_bits=bits, master=True)
+        names = ["m", "v", "master"] + (["m_scale", "v_scale"] if bits == 8 else [])
+        old = {name: list(getattr(plan, name)) for name in names}              # (kept, so that nothing is freed)
+        before = [p.clone() for p in params]
+        for name in names:
+            getattr(plan, name)[1] = old[name][1].clone()
+            with pytest.raises(RuntimeError, match=name):
+                plan.step(grads, rate=1e-2, t=1)
+            getattr(plan, name)[1] = old[name][1]
+            setattr(plan, name, [t.clone() for t in old[name]])
+            with pytest.raises(RuntimeError, match=name):
+                plan.step(grads, rate=1e-2, t=1)
+            setattr(plan, name, old[name][:1])
+            with pytest.raises(RuntimeError, match=name):
+                plan.step(grads, rate=1e-2, t=1)
+            setattr(plan, name, list(old[name]))
+            memory = old[name][0].data
+            old[name][0].data = memory.clone()
+            with pytest.raises(RuntimeError, match=name):
+                plan.step(grads, rate=1e-2, t=1)
+            old[name][0].data = memory
+        assert all(torch.equal(p, b) for p, b in zip(params, before))
+        plan.step(grads, rate=1e-2, t=1)
+        assert not torch.equal(params[0], before[0])
+        plan.m[0].copy_(torch.zeros_like(plan.m[0].float()))
+        plan.step(grads, rate=1e-2, t=2)
