@@ -757,7 +757,7 @@ typedef struct pxe_adamw_desc {
     float rate, beta1, beta2, eps, weight_decay, grad_scale;
     long long t;               /* counts steps from 1 */
     /* device scalars that replace the values above when they are not NULL (a step captured in a CUDA graph reads the
-     * current ones at every replay), and a flag that, not 0, leaves everything as it is */
+     * current ones at every replay; a t below 1 leaves everything as it is), and a flag that, not 0, does so too */
     const float* rate_device;
     const long long* t_device;
     const float* grad_scale_device;

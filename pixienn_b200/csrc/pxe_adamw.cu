@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, SMALL && sizeof(P) == 2 ? 6 : 4)
 adamw_kernel(const __grid_constant__ AdamwParams<MAX> a)
 {
     if (a.skip_device && gld(a.skip_device) != 0.0f) return;
+    if (a.t_device && gld(a.t_device) < 1) return;         // 1 - b^0 = 0 would divide
     // chosen as values: a member of Step overwritten under a condition kept the parameter's value (nvcc 12.9)
     const float rate = a.rate_device ? gld(a.rate_device) : a.rate;
     const float grad_scale = a.grad_scale_device ? gld(a.grad_scale_device) : a.grad_scale;

@@ -1220,7 +1220,8 @@ class AdamW:
         """One step, in place on the parameters and the state.  ``grads``: one contiguous tensor for each parameter, all
         of one type (float32 or the parameters' own; any of the three types for float32 parameters).  ``t`` counts steps
         from 1.  ``rate``, ``grad_scale`` (float32) and ``t`` (int64) may be CUDA tensors of one element, which a captured
-        step reads at every replay; ``skip``: a float32 one that, not 0, makes the step do nothing."""
+        step reads at every replay; a ``t`` below 1 there makes the step do nothing, and so does ``skip``, a float32 one,
+        when it is not 0."""
         count = len(self._sizes)
         if len(grads) != count:
             raise ValueError(f"{len(grads)} gradients for {count} parameters")

@@ -126,3 +126,19 @@ def test_adamw_refuses_a_state_that_was_replaced(cuda):
         assert not torch.equal(params[0], before[0])
         plan.m[0].copy_(torch.zeros_like(plan.m[0].float()))
         plan.step(grads, rate=1e-2, t=2)
+
+
+def test_adamw_counter_below_one_leaves_everything(cuda):
+    """t counts from 1; a device counter that is not there yet (a step replayed before it is raised) changes nothing, where
+    1 - beta^0 = 0 would divide."""
+    for bits in (32, 8):
+        params, grads = [rand(710, (300,)), rand(711, (5,))], [rand(712, (300,)), rand(713, (5,))]
+        plan = ops.AdamW(params, state_bits=bits)
+        plan.step(grads, rate=1e-2, t=1)
+        held = params + plan.m + plan.v + (plan.m_scale + plan.v_scale if bits == 8 else [])
+        before = [x.clone() for x in held]
+        for t in (0, -1, -(1 << 40)):
+            plan.step(grads, rate=1e-2, t=torch.tensor([t], device="cuda"))
+            assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(held, before))
+        plan.step(grads, rate=1e-2, t=torch.tensor([2], device="cuda"))
+        assert not torch.equal(params[0], before[0]) and bool(params[0].isfinite().all())
