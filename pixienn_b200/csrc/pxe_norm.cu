@@ -582,12 +582,13 @@ rms_norm_backward_long_kernel(const NormBackParams p)
 // A block has to go over many rows (its part of dweight is in its registers), and the form above waits for one row while it
 // works on another: too few bytes are on their way (a row's chain of load, barrier, reduction and store takes about 1.5 us,
 // whatever it moves).  Here one thread keeps `stages` rows of every input coming in with bulk copies.  A row's barrier in
-// its reduction says that all threads are done with the row before, whose place is then refilled.  Waits are bounded: a
-// copy that never completes leaves NaN behind, not a hang.  16384 x 4096 bf16: 82 us, the copy rate, against 91 by the form
+// its reduction says that all threads are done with the row before, whose place is then refilled.  Waits are bounded: where a
+// copy does not complete, the block leaves NaN in that row of dx, in all its later ones and in its part of dweight, starts
+// no further copy, and waits, bounded too, for those under way, which end in its shared memory.  16384 x 4096 bf16: 82 us, the copy rate, against 91 by the form
 // above; 4096 x 8192: 46 against 74; 16384 x 1024: 27.4 against 27.9.  (Several short rows to a stage, filled by a warp, were
 // slower than the form above: 44 against 28 us at 8192 x 2048.)
 constexpr int kMaxStages = 8;
-constexpr int kWaitLimit = 1 << 20;
+constexpr int kWaitLimit = 1 << 18;                        // tries of 4 us each: about a second
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -638,15 +639,17 @@ struct Ring {
 extern __shared__ __align__(128) unsigned char ring_shared[];
 
 template <typename T>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(1024, 1)                   // (an SM holds 1024 threads of any of its blocks: 64 registers each)
 rms_norm_backward_ring_kernel(const NormBackParams p, int stages)
 {
     constexpr int VEC = 16 / sizeof(T);                    // a thread holds one vector of the row
     __shared__ float reds[2][32];
     __shared__ unsigned long long full[kMaxStages];
+    __shared__ int missing[2];                             // a thread's wait ran out (alternating as reds do)
     const int C = p.channels, col = threadIdx.x * VEC, bytes = C * (int)sizeof(T), inputs = p.dres ? 3 : 2;
     const bool there = col < C;
     const Ring ring{ring_shared, full, stages, bytes * inputs};
+    if (threadIdx.x < 2) missing[threadIdx.x] = 0;
     ring.init();
     auto fill = [&](int stage, long long row) {
         const void* const src[3] = {static_cast<const T*>(p.dy) + row * p.dys, static_cast<const T*>(p.h) + row * p.hs, static_cast<const T*>(p.dres) + row * p.rs};
@@ -662,18 +665,20 @@ rms_norm_backward_ring_kernel(const NormBackParams p, int stages)
     if (there) load_weight<T, VEC>(p.weight, p.weight_f32, col, w);
     float next_rstd = gld(p.rstd + blockIdx.x);            // (there are at least two rows for each block)
     int stage = 0, parity = 0, turn = 0;
-    for (long long row = blockIdx.x; row < p.rows; row += step, turn ^= 1) {
+    long long row = blockIdx.x;
+    for (; row < p.rows; row += step, turn ^= 1) {
         const float rstd = next_rstd;
         if (row + step < p.rows) next_rstd = gld(p.rstd + row + step);
-        const bool arrived = ring.wait(stage, parity);
+        if (!ring.wait(stage, parity)) missing[turn] = 1;
         const unsigned char* const at = ring.data + stage * ring.stage_bytes + col * (int)sizeof(T);
-        float dot = arrived ? 0.0f : __int_as_float(0x7fffffff);
+        float dot = 0.0f;
         if (there) {
             unpack<T, VEC>(ring.read<Raw<T, VEC>>(at), u);
             unpack<T, VEC>(ring.read<Raw<T, VEC>>(at + bytes), h);
             dot = first_pass<T, VEC>(u, h, w, rstd, acc[0], dot);
         }
         dot = row_reduce<false>(dot, reds[turn]);
+        if (missing[turn]) break;                          // the same for all: written before the barrier, or two rows later
         const int before = stage == 0 ? stages - 1 : stage - 1;
         if (threadIdx.x == 0 && row != blockIdx.x && row + (stages - 1) * step < p.rows) fill(before, row + (stages - 1) * step);
         if (there) {
@@ -685,6 +690,15 @@ rms_norm_backward_ring_kernel(const NormBackParams p, int stages)
             gstv(static_cast<T*>(p.dx) + row * p.dxs + col, pack<T, VEC>(u));
         }
         if (++stage == stages) { stage = 0; parity ^= 1; }
+    }
+    if (row < p.rows) {                                    // given up
+        // under way: this row's copies and the next rows', as far as they were started (from the first row, one more)
+        const int started = row == blockIdx.x ? stages : stages - 1;
+        if (threadIdx.x == 0)
+            for (int i = 0; i < started && row + i * step < p.rows; ++i) ring.wait((stage + i) % stages, parity ^ (stage + i >= stages));
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[0][j] = u[j] = __int_as_float(0x7fffffff);
+        for (; there && row < p.rows; row += step) gstv(static_cast<T*>(p.dx) + row * p.dxs + col, pack<T, VEC>(u));
     }
     if (p.partial) store_partial<VEC, 1>(acc, p.partial + (long long)blockIdx.x * C, C, col, nullptr);
 }
