@@ -142,3 +142,17 @@ def test_adamw_counter_below_one_leaves_everything(cuda):
             assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(held, before))
         plan.step(grads, rate=1e-2, t=torch.tensor([2], device="cuda"))
         assert not torch.equal(params[0], before[0]) and bool(params[0].isfinite().all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("rate,decay", [(1e-4, 0.01), (3e-6, 0.1), (1e-3, 0.05)])
+def test_adamw_decay_of_few_units_is_not_quantised(cuda, bits, rate, decay):
+    """With nothing but decay (gradient and moments 0) the parameter is p - rate decay p, rounded once: off by half of its own
+    step, and U of the decay itself for each of its two products, whatever rate * decay is next to 2^-24."""
+    p = rand(720, (20000,))
+    plan, before = ops.AdamW([p], state_bits=bits), p.double()
+    plan.step([torch.zeros_like(p)], rate=rate, t=1, weight_decay=decay)
+    shrink = float(torch.tensor(rate, dtype=torch.float32).double() * torch.tensor(decay, dtype=torch.float32).double())
+    want = before * (1 - shrink)
+    step = (torch.nextafter(p.abs(), torch.full_like(p, INF)) - p.abs()).double()
+    within(p, want, step / 2 + 2 * U * shrink * before.abs())
