@@ -173,7 +173,7 @@ class AdamwDesc(C.Structure):
     _fields_ = [("tensors", C.c_void_p), ("count", C.c_int), ("param_type", C.c_int), ("grad_type", C.c_int), ("state_bits", C.c_int),
                 ("rate", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float), ("weight_decay", C.c_float),
                 ("grad_scale", C.c_float), ("t", C.c_longlong), ("rate_device", C.c_void_p), ("t_device", C.c_void_p),
-                ("grad_scale_device", C.c_void_p), ("skip_device", C.c_void_p)]
+                ("grad_scale_device", C.c_void_p), ("skip_device", C.c_void_p), ("seed", C.c_ulonglong)]
 
 
 ADAMW_BLOCK = 256                         # PXE_ADAMW_BLOCK

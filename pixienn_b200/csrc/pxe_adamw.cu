@@ -12,7 +12,9 @@
 //
 // In 8 bits m is held as an e4m3 code times its block's scale, and v as the code of its root: the update needs the root,
 // and its codes then reach 2^-18 of the block's largest value (2^-36 in v).  A v above zero keeps the smallest code
-// instead of rounding to zero, which would leave a later step to divide by eps alone.
+// instead of rounding to zero, which would leave a later step to divide by eps alone.  Codes are 6 to 12 % apart, and a step
+// moves the root of v by 0.05 % (beta2 = 0.999): rounded to nearest, all of that is lost and the moments stand still.
+// With a seed they are rounded up or down at random, each as likely as it is near, so that on average nothing is lost.
 #include <algorithm>
 #include <exception>
 #include <type_traits>
@@ -47,7 +49,9 @@ struct AdamwParams {
     const long long* t_device;
     const float* grad_scale_device;
     const float* skip_device;
-    int count, blocks;
+    unsigned long long seed;
+    long long t;
+    int count, blocks, before;                             // tensors of this launch, their blocks, tensors of earlier launches
     Entry e[MAX];
 };
 
@@ -80,6 +84,27 @@ struct Step {
         return r;
     }
 };
+
+// A 32-bit integer hash: C. Wellons, "Prospecting for hash functions" (2018), the variant with two multiplications.
+__device__ __forceinline__ uint32_t mix(uint32_t x)
+{
+    x ^= x >> 16;
+    x *= 0x7feb352du;
+    x ^= x >> 15;
+    x *= 0x846ca68bu;
+    return x ^ x >> 16;
+}
+__device__ __forceinline__ uint32_t mix(uint32_t x, unsigned long long next) { return mix(mix(x ^ (uint32_t)next) ^ (uint32_t)(next >> 32)); }
+
+// a in [0, 448) to the e4m3 value below or above it by 16 random bits: they are added under the three bits of the mantissa
+// that a code has (among the smallest codes, 2^-9 apart, after 2^-6 is added, where floats have those bits at 2^-9), and
+// what lies under the three is cut off.  Too likely by 2^-17 at most.  Anything else as it is, for the conversion to round.
+__device__ __forceinline__ float round_at_random(float a, uint32_t bits16)
+{
+    const float base = a < 0.015625f ? 0.015625f : 0.0f;
+    const float q = __uint_as_float((__float_as_uint(a + base) + (bits16 << 4)) & 0xfff00000u) - base;
+    return a < kE4m3Max ? fminf(q, kE4m3Max) : a;
+}
 
 __device__ __forceinline__ float warp_max(float v)
 {
@@ -127,8 +152,9 @@ __device__ __forceinline__ void store(T* p, const float (&f)[N])
     }
 }
 
-// One unit of 256 elements of a warp: all its loads, then the work on them.
-template <typename P, typename G, bool SMALL, bool MASTER, int N>
+// One unit of 256 elements of a warp: all its loads, then the work on them.  RANDOM: 8-bit codes are rounded at random, by a
+// hash of `key` (of seed, step, tensor and unit) and the element's place in the unit.
+template <typename P, typename G, bool SMALL, bool RANDOM, bool MASTER, int N>
 struct Unit {
     using S = std::conditional_t<SMALL, uint8_t, float>;
     using W = std::conditional_t<MASTER, float, P>;
@@ -150,7 +176,7 @@ struct Unit {
         v.load(static_cast<const S*>(e.v) + at, left);
         if constexpr (SMALL) { ms = gld(e.ms + first / kUnit); vs = gld(e.vs + first / kUnit); }
     }
-    __device__ __forceinline__ void work(const Entry& e, long long first, int lane, const Step& step)
+    __device__ __forceinline__ void work(const Entry& e, long long first, int lane, const Step& step, uint32_t key)
     {
         float m1[COUNT][N], v1[COUNT][N], m_max = 0.0f, v_max = 0.0f;
 #pragma unroll
@@ -197,7 +223,13 @@ struct Unit {
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     m1[k][j] *= mi;
-                    v1[k][j] = v1[k][j] > 0.0f ? max_nan(v1[k][j] * vi, kSmallest) : v1[k][j];
+                    float r = v1[k][j] * vi;
+                    if constexpr (RANDOM) {
+                        const uint32_t h = mix(key ^ (uint32_t)(lane * N + k * STRIDE + j));
+                        m1[k][j] = copysignf(round_at_random(fabsf(m1[k][j]), h & 0xffffu), m1[k][j]);
+                        r = round_at_random(r, h >> 16);
+                    }
+                    v1[k][j] = v1[k][j] > 0.0f ? max_nan(r, kSmallest) : v1[k][j];
                 }
                 if (k * STRIDE < left) {
                     gstv(static_cast<uint8_t*>(e.m) + at + k * STRIDE, pack_e4m3<N>(m1[k]));
@@ -208,21 +240,21 @@ struct Unit {
     }
 };
 
-template <typename P, typename G, bool SMALL, bool MASTER, int N>
-__device__ __forceinline__ void one_unit(const Entry& e, long long first, int lane, const Step& step)
+template <typename P, typename G, bool SMALL, bool RANDOM, bool MASTER, int N>
+__device__ __forceinline__ void one_unit(const Entry& e, long long first, int lane, const Step& step, uint32_t key)
 {
-    Unit<P, G, SMALL, MASTER, N> u;
+    Unit<P, G, SMALL, RANDOM, MASTER, N> u;
     u.load(e, first, lane);
-    u.work(e, first, lane, step);
+    u.work(e, first, lane, step, key);
 }
 
 // 64 M elements: fp32 with states in 32 bits 272 us, 1.07 of the copy rate; fp32 with states in 8 bits 158 us (1.06); bf16
-// with a master copy and states in 8 bits 164 us (1.01), without the copy 123 us (0.85, 12 bytes an element and as many
-// instructions).
+// with a master copy and states in 8 bits 158 us (1.06), without the copy 126 us (0.83, 12 bytes an element and as many
+// instructions).  With a seed 223, 208 and 204 us: bound by the instructions of the hash and the roundings.
 // Blocks of an SM: four (64 registers a thread, nothing spilled), six for 16-bit parameters with states in 8 bits, whose
 // lanes have half the bytes under way (64 M bf16 parameters: 122 against 134 us, with a master copy 164 against 167; fp32
 // parameters with states in 8 bits 157 against 171 us at six).
-template <typename P, typename G, bool SMALL, bool MASTER, int MAX>
+template <typename P, typename G, bool SMALL, bool RANDOM, bool MASTER, int MAX>
 __global__ void __launch_bounds__(kThreads, SMALL && sizeof(P) == 2 ? 6 : 4)
 adamw_kernel(const __grid_constant__ AdamwParams<MAX> a)
 {
@@ -248,27 +280,37 @@ adamw_kernel(const __grid_constant__ AdamwParams<MAX> a)
     const Entry& e = a.e[lo];
     const long long first = (long long)((int)blockIdx.x - e.first_block) * kElements + warp * kUnit;
     if (first >= e.n) return;
-    if (e.vector && first + kUnit <= e.n) one_unit<P, G, SMALL, MASTER, N>(e, first, lane, step);
-    else one_unit<P, G, SMALL, MASTER, 1>(e, first, lane, step);
+    uint32_t key = 0;
+    if constexpr (RANDOM) {
+        const long long t = a.t_device ? gld(a.t_device) : a.t;
+        key = mix(mix(mix(mix(0u, a.seed), (unsigned long long)t), (unsigned long long)(a.before + lo)), (unsigned long long)(first / kUnit));
+    }
+    if (e.vector && first + kUnit <= e.n) one_unit<P, G, SMALL, RANDOM, MASTER, N>(e, first, lane, step, key);
+    else one_unit<P, G, SMALL, RANDOM, MASTER, 1>(e, first, lane, step, key);
 }
 
-template <typename P, typename G, bool SMALL, bool MASTER>
-int launch(cudaStream_t s, AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>& a)
+using Params = AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>;
+
+template <typename P, typename G, bool SMALL, bool RANDOM, bool MASTER>
+int launch(cudaStream_t s, const Params& a)
 {
-    adamw_kernel<P, G, SMALL, MASTER, PXE_ADAMW_TENSORS_PER_LAUNCH><<<(unsigned)a.blocks, kThreads, 0, s>>>(a);
+    adamw_kernel<P, G, SMALL, RANDOM, MASTER, PXE_ADAMW_TENSORS_PER_LAUNCH><<<(unsigned)a.blocks, kThreads, 0, s>>>(a);
     PXE_LAUNCH_OK("adamw_kernel");
     return PXE_OK;
 }
 
-template <typename P, typename G>
-int launch(cudaStream_t s, AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH>& a, bool small, bool master)
+template <typename P, typename G, bool MASTER>
+int launch(cudaStream_t s, const Params& a, bool small)
 {
-    if constexpr (sizeof(P) == 4) {
-        return small ? launch<P, G, true, false>(s, a) : launch<P, G, false, false>(s, a);
-    } else {
-        if (master) return small ? launch<P, G, true, true>(s, a) : launch<P, G, false, true>(s, a);
-        return small ? launch<P, G, true, false>(s, a) : launch<P, G, false, false>(s, a);
-    }
+    if (!small) return launch<P, G, false, false, MASTER>(s, a);
+    return a.seed ? launch<P, G, true, true, MASTER>(s, a) : launch<P, G, true, false, MASTER>(s, a);
+}
+
+template <typename P, typename G>
+int launch(cudaStream_t s, const Params& a, bool small, bool master)
+{
+    if constexpr (sizeof(P) == 2) { if (master) return launch<P, G, true>(s, a, small); }
+    return launch<P, G, false>(s, a, small);
 }
 
 struct Range {
@@ -306,6 +348,7 @@ extern "C" int pxe_adamw_update(pxe_stream_t stream, const pxe_adamw_desc* dp)
     if (d.param_type != PXE_F32 && d.grad_type != d.param_type && d.grad_type != PXE_F32)
         return set_error(PXE_ERR_UNSUPPORTED, "adamw_update: gradients of one 16-bit type for parameters of the other");
     PXE_REQUIRE(d.state_bits == 32 || d.state_bits == 8, "adamw_update: state_bits %d is neither 32 nor 8", d.state_bits);
+    PXE_REQUIRE(d.seed == 0 || d.state_bits == 8, "adamw_update: a seed rounds states in 8 bits only");
     PXE_REQUIRE(d.beta1 >= 0.0f && d.beta1 < 1.0f && d.beta2 >= 0.0f && d.beta2 < 1.0f, "adamw_update: beta1 and beta2 lie in [0, 1)");
     PXE_REQUIRE(d.eps >= 0.0f, "adamw_update: eps is negative or NaN");
     PXE_REQUIRE(d.t_device || d.t >= 1, "adamw_update: step %lld (the first step is 1)", d.t);
@@ -348,16 +391,17 @@ extern "C" int pxe_adamw_update(pxe_stream_t stream, const pxe_adamw_desc* dp)
         return set_error(PXE_ERR_CUDA, "adamw_update: %s", e.what());
     }
     if (first) return PXE_OK;                              // nothing to do
-    AdamwParams<PXE_ADAMW_TENSORS_PER_LAUNCH> a;
+    Params a;
     a.rate = d.rate; a.b1 = d.beta1; a.b2 = d.beta2; a.omb1 = (float)(1.0 - (double)d.beta1); a.omb2 = (float)(1.0 - (double)d.beta2);
     a.eps = d.eps; a.decay = d.weight_decay; a.grad_scale = d.grad_scale;
     a.log_b1 = (float)std::log((double)d.beta1); a.log_b2 = (float)std::log((double)d.beta2);
     a.inv_c1 = d.t_device ? 0.0f : (float)(1.0 / (1.0 - std::pow((double)d.beta1, (double)d.t)));
     a.inv_c2 = d.t_device ? 0.0f : (float)(1.0 / (1.0 - std::pow((double)d.beta2, (double)d.t)));
     a.rate_device = d.rate_device; a.t_device = d.t_device; a.grad_scale_device = d.grad_scale_device; a.skip_device = d.skip_device;
+    a.seed = d.seed; a.t = d.t; a.before = 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int i = 0;
-    while (i < d.count) {
+    for (; i < d.count; a.before += a.count) {
         a.count = 0;
         long long blocks = 0;
         for (; i < d.count && a.count < PXE_ADAMW_TENSORS_PER_LAUNCH; ++i) {

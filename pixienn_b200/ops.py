@@ -1136,15 +1136,21 @@ class AdamW:
 
     ``params``: contiguous CUDA tensors of one type (float32, bfloat16 or float16) on one device.  ``state_bits=32``
     keeps ``m`` and ``v`` as float32; ``state_bits=8`` keeps ``m`` and the root of ``v`` as float8_e4m3fn codes with a
-    float32 scale for every 256 elements (``m_scale``, ``v_scale``).  ``master=True`` keeps float32 copies of 16-bit
+    float32 scale for every 256 elements (``m_scale``, ``v_scale``).  Codes are 6 to 12 % apart: rounded to nearest, as
+    they are without a ``seed``, they lose what a step moves by less, and over many steps the moments stop following the
+    gradients.  Training takes a ``seed`` (a whole number above 0): codes are then rounded up or down at random, so that
+    on average nothing is lost, and the same steps with the same seed give the same bits.  ``master=True`` keeps float32 copies of 16-bit
     parameters and updates those.  All are lists, one tensor for each parameter; lists of an earlier state can be given
     instead (a loaded checkpoint) and are then updated in place.  The plan holds the parameters and the state; a tensor
     of either that was replaced, or whose memory has moved since, is refused by :meth:`step`.  To load another state
     later, copy into the tensors or make a new plan."""
 
-    def __init__(self, params: Sequence[torch.Tensor], *, state_bits: int = 32, m=None, v=None, m_scale=None, v_scale=None, master=None):
+    def __init__(self, params: Sequence[torch.Tensor], *, state_bits: int = 32, m=None, v=None, m_scale=None, v_scale=None, master=None,
+                 seed: Optional[int] = None):
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if seed is not None and (state_bits != 8 or not 0 < seed < 1 << 64):
+            raise ValueError(f"seed must be a whole number from 1 to 2^64 - 1, for states in 8 bits, got {seed} for {state_bits}")
         self.params = list(params)
         self.state_bits = state_bits
         self._dtype, self._device = torch.float32, None
@@ -1191,6 +1197,7 @@ class AdamW:
         self._grads = column("grad")
         d = self._desc = capi.AdamwDesc()
         d.tensors, d.count, d.state_bits, d.param_type = self._table.ctypes.data, count, state_bits, _DTYPE[self._dtype]
+        d.seed = seed or 0
 
     def _state(self, given, sizes, dtype, name):
         if given is None:                    # one buffer, every tensor on a 256-byte boundary

@@ -156,3 +156,122 @@ def test_adamw_decay_of_few_units_is_not_quantised(cuda, bits, rate, decay):
     want = before * (1 - shrink)
     step = (torch.nextafter(p.abs(), torch.full_like(p, INF)) - p.abs()).double()
     within(p, want, step / 2 + 2 * U * shrink * before.abs())
+
+
+def decoded(codes, scale):
+    return codes.double() * scale.double().repeat_interleave(256)[:codes.numel()]
+
+
+@pytest.mark.parametrize("dtype,gtype", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16),
+                                         (torch.bfloat16, torch.float32), (torch.float16, torch.float16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("master", [False, True])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_adamw_seeded_codes_are_neighbours_and_fair(cuda, dtype, gtype, master, shift):
+    """With a seed each code is the value's neighbour above or below, and their mean error is none: that of n values is within
+    five times 1/2 step / sqrt(n) (a code's error has a deviation of at most half a step), and 2^-17 of a step for 16 random
+    bits.  Everything else is as without a seed."""
+    if master and dtype == torch.float32:
+        return
+    sizes = [200003, 77, 512]
+    made = lambda s: [rand(s + k, (n + shift,), dtype, 0.05)[shift:] for k, n in enumerate(sizes)]  # noqa: E731
+    grads = [[rand(s + k, (n + shift,), gtype, 0.01)[shift:] for k, n in enumerate(sizes)] for s in (740, 750)]
+    a, b = made(730), made(730)
+    pa, pb = ops.AdamW(a, state_bits=8, master=master, seed=5), ops.AdamW(b, state_bits=8, master=master)
+    pa.step(grads[0], rate=1e-2, t=1)
+    pb.step(grads[0], rate=1e-2, t=1)
+    assert all(torch.equal(x, y) for x, y in zip(a + pa.m_scale + pa.v_scale, b + pb.m_scale + pb.v_scale))
+    b1, b2 = (float(torch.tensor(x, dtype=torch.float32)) for x in (0.9, 0.999))
+    m0, r0 = ([decoded(q, s) for q, s in zip(*z)] for z in ((pa.m, pa.m_scale), (pa.v, pa.v_scale)))
+    pa.step(grads[1], rate=1e-2, t=2)
+    errors = []
+    for k, n in enumerate(sizes):
+        g = grads[1][k].double()
+        for q, s, want in ((pa.m[k], pa.m_scale[k], b1 * m0[k] + (1 - b1) * g),
+                           (pa.v[k], pa.v_scale[k], (b2 * r0[k].square() + (1 - b2) * g * g).sqrt())):
+            each = s.double().repeat_interleave(256)[:n]
+            at = (want / each).abs()
+            step = torch.exp2(torch.floor(torch.log2(at.clamp(min=2.0 ** -6))) - 3)          # between codes around the value
+            # a neighbour: less than a step away, 16 U of the value for what is computed on the way, which can lie over a
+            # code's value itself (an error of a whole step of the next octave: twice as long)
+            off = (decoded(q, s) - want) / each
+            floor = (q is pa.v[k]) & (at < 2.0 ** -9)                                        # kept at the smallest code
+            assert bool((off.abs() <= torch.where(floor, 2.0 ** -9, step) + 2 * step * (at * 16 * U > step * 2.0 ** -17) + at * 16 * U).all())
+            if n > 100000:
+                errors.append((off / step * want.sign())[(at > 2.0 ** -6) & (at < 448 * 0.999)])
+        assert bool(((pa.v[k].float() > 0) == (r0[k].square() + g * g > 0)).all())
+    for e in errors:
+        assert abs(float(e.mean())) <= 2.5 / math.sqrt(e.numel()) + 2.0 ** -17 + 1e-4
+        assert 0.1 < float(e.abs().mean()) < 0.5              # (to nearest it is at most 0.25; at random the mean of 2 f (1 - f) is 1/3)
+
+
+def test_adamw_seeded_steps_repeat_and_differ(cuda):
+    """The same bits for the same seed, t and places, whatever the alignment and however t is given; others for another seed,
+    t or tensor."""
+    n = 5000
+    def state(seed, t, device_t=False, shift=0, count=2):
+        params = [rand(760, (n + shift,))[shift:].clone() if not shift else rand(760, (n,)).clone() for _ in range(count)]
+        if shift:
+            params = [torch.empty(n + shift, device="cuda")[shift:].copy_(p) for p in params]
+        plan = ops.AdamW(params, state_bits=8, seed=seed)
+        grads = [rand(761, (n,), scale=0.01) for _ in range(count)]
+        plan.step(grads, rate=1e-3, t=torch.tensor([t], device="cuda") if device_t else t)
+        return [x.float() for x in plan.m + plan.v]
+    one = state(7, 3)
+    same = lambda a, b: all(torch.equal(x, y) for x, y in zip(a, b))  # noqa: E731
+    assert same(one, state(7, 3)) and same(one, state(7, 3, device_t=True)) and same(one, state(7, 3, shift=1))
+    many = state(7, 3, count=450)                             # more than one launch
+    assert same(one[:2], many[:2]) and same(one[2:], many[450:452])
+    assert not torch.equal(many[0], many[1]) and not torch.equal(many[399], many[400]) and not torch.equal(many[0], many[400])
+    for other in (state(8, 3), state(7 + (1 << 32), 3), state(7, 4), state(7, 3 + (1 << 32))):
+        assert 0.05 < float((other[0] != one[0]).float().mean()) < 0.95
+    for bad in (0, -1, 1 << 64):
+        with pytest.raises(ValueError):
+            ops.AdamW([torch.zeros(4, device="cuda")], state_bits=8, seed=bad)
+    with pytest.raises(ValueError):
+        ops.AdamW([torch.zeros(4, device="cuda")], seed=1)
+
+
+def test_adamw_seeded_state_keeps_what_is_not_finite_and_zero(cuda):
+    """A gradient of 0 on a fresh state leaves zeros; one that is not finite spoils its block and no other, as without a seed."""
+    p = [rand(770, (1024,))]
+    plan = ops.AdamW(p, state_bits=8, seed=3)
+    plan.step([torch.zeros(1024, device="cuda")], rate=1e-3, t=1)
+    assert bool((plan.m[0].float() == 0).all()) and bool((plan.v[0].float() == 0).all())
+    for bad in (float("nan"), INF, -INF):
+        q = [p[0].clone()]
+        plan, plain = ops.AdamW(q, state_bits=8, seed=3), ops.AdamW([p[0].clone()], state_bits=8)
+        g = rand(771, (1024,))
+        g[300] = bad
+        plan.step([g], rate=1e-3, t=1)
+        plain.step([g], rate=1e-3, t=1)
+        for x, y in ((plan.m[0], plain.m[0]), (plan.v[0], plain.v[0])):
+            assert torch.equal(x.float().isnan(), y.float().isnan()) and not bool(x[:256].float().isnan().any() | x[512:].float().isnan().any())
+        assert torch.equal(q[0].isnan(), plain.params[0].isnan())
+
+
+def test_adamw_long_run_of_seeded_8_bit_state_follows_32_bits(cuda):
+    """1300 steps of gradients whose sizes spread over orders of magnitude within a block; after 300 those of every other
+    element fall to a tenth.  The root of v of 8-bit state over that of 32-bit state: a code's error is fair, so that the mean
+    over many elements is off by half of the ratio's variance at most.  That variance: what rounding adds each step, |move| *
+    code step, over twice the rate 1 - beta2 at which v forgets: a move of about (1 - beta2) / 2 of the root for what the
+    gradient says and as much for the scale's own, codes 1/8 apart at most: 1/16 and a little more where gradients have fallen.
+    So: mean within 8 %, 90 % of the elements within a factor of 2.  (To nearest the fallen half is 2.0 times too large
+    after these 1000 steps and 6.8 after 4000, the other at 0.77 of what it should be.)"""
+    n = 64 * 256
+    size = torch.exp(rand(780, (n,))) * 0.01
+    a, b = [torch.zeros(n, device="cuda")], [torch.zeros(n, device="cuda")]
+    small, wide = ops.AdamW(a, state_bits=8, seed=11), ops.AdamW(b)
+    g = gen(781)
+    for t in range(1, 1301):
+        if t == 301:
+            size[::2] *= 0.1
+        grad = [torch.randn(n, device="cuda", generator=g) * size]
+        small.step(grad, rate=1e-4, t=t)
+        wide.step(grad, rate=1e-4, t=t)
+        if t in (300, 800, 1300):
+            ratio = decoded(small.v[0], small.v_scale[0]) / wide.v[0].double().sqrt()
+            for part in (ratio[::2], ratio[1::2]):
+                assert 0.92 <= float(part.mean()) <= 1.08
+                assert float(torch.quantile(part, 0.05)) >= 0.5 and float(torch.quantile(part, 0.95)) <= 2.0
+    # both have moved the parameters alike: the sum of 1300 updates of a rate each
+    assert float((a[0] - b[0]).double().norm() / b[0].double().norm()) <= 0.25

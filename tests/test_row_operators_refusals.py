@@ -27,3 +27,8 @@ def test_adamw_refuses_device_scalars_inside_what_it_writes():
     refused(adamw([{}, {"param": E, "grad": B_ + 8000, "m": C_ + 8000, "v": F}], t_device=F + 3992), "device scalar")
     refused(adamw([{"m_scale": E, "v_scale": F}], state_bits=8, rate_device=F + 12), "device scalar")
     refused(adamw([{"master": E}], param_type=capi.BF16, grad_type=capi.BF16, skip_device=E), "device scalar")
+
+
+def test_adamw_seed_comes_with_8_bit_state():
+    refused(adamw([{}], seed=1), "seed")
+    refused(adamw([{"m_scale": E, "v_scale": F, "m": C_ + 2, "grad": A}], state_bits=8, seed=1), "overlap")        # (past the seed's check)
