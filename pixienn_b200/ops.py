@@ -827,10 +827,14 @@ def softmax_cross_entropy(pred: torch.Tensor, truth: torch.Tensor):
 # ------------------------------------------------------------------------------ row operators in 32- and 16-bit types
 # A call on a token's row is as long as its marshalling: what holds is checked in line, a property at a time, and the
 # functions below that word a refusal are called only where something does not.
+# The operators are no autograd functions: what they return has no graph, and each gradient is a call of its own.  A graph
+# that saved a tensor which a call writes in place finds that out from its version, which the call raises (a replayed
+# capture does not).
 _DTYPE = {torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16}
 _raw_stream = torch._C._cuda_getCurrentRawStream          # of a device's index; what current_stream(...).cuda_stream reads
 _current_device = torch._C._cuda_getDevice
 _data_ptr = torch.Tensor.data_ptr
+_written = torch.autograd.graph.increment_version         # of one tensor or several
 _f32 = torch.float32
 
 
@@ -965,6 +969,10 @@ def _rms_norm(x, weight, residual, eps, out, residual_out, e4m3, group):
         rc = capi.lib().pxe_rms_norm(_raw_stream(dev), C.byref(d))
         if rc:
             capi.check(rc)
+        if out is not None:
+            _written(y)
+        if residual_out is not None:
+            _written(h)
     return y, scale, h, rstd
 
 
@@ -1012,6 +1020,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.
     if dresidual is not None:
         _like(dresidual, shape, dtype, dev, "dresidual")
         rp, rs = dresidual.data_ptr(), _row_stride(dresidual, "dresidual")
+    given_dx = dx
     if dx is None:
         dx, dxs = torch.empty_like(dy, memory_format=torch.contiguous_format), channels
     else:
@@ -1032,6 +1041,10 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.
     rc = lib.pxe_rms_norm_backward(_raw_stream(dev), C.byref(d))
     if rc:
         capi.check(rc)
+    if given_dx is not None:
+        _written(dx)
+    if accumulate:
+        _written(dweight)
     return dx, dweight
 
 
@@ -1115,7 +1128,8 @@ def log_probs_backward(x: torch.Tensor, target: Optional[torch.Tensor], stats: t
     if dlogp is not None and target is None:
         raise ValueError("dlogp without target")
     tp, is64 = _target(target, shape[:-1], dev) if target is not None else (None, 0)
-    if dx is None:
+    given = dx is not None
+    if not given:
         dx = torch.empty_strided(shape, x.stride(), device=x.device, dtype=dtype)
         inner, outer, stride = (0, 0, classes) if x.is_contiguous() else _grouped_rows(x, "x")
         dx_outer, dx_stride = outer, stride
@@ -1128,6 +1142,8 @@ def log_probs_backward(x: torch.Tensor, target: Optional[torch.Tensor], stats: t
     rc = capi.lib().pxe_log_probs_backward(_raw_stream(dev), C.byref(d))
     if rc:
         capi.check(rc)
+    if given:
+        _written(dx)
     return dx
 
 
@@ -1271,3 +1287,4 @@ class AdamW:
             d.skip_device = self._scalar(skip, torch.float32, "skip")
         d.beta1, d.beta2, d.eps, d.weight_decay = beta1, beta2, eps, weight_decay
         capi.check(capi.lib().pxe_adamw_update(_raw_stream(dev), C.byref(d)))
+        _written(self.params)

@@ -275,3 +275,45 @@ def test_adamw_long_run_of_seeded_8_bit_state_follows_32_bits(cuda):
                 assert float(torch.quantile(part, 0.05)) >= 0.5 and float(torch.quantile(part, 0.95)) <= 2.0
     # both have moved the parameters alike: the sum of 1300 updates of a rate each
     assert float((a[0] - b[0]).double().norm() / b[0].double().norm()) <= 0.25
+
+
+# ------------------------------------------------------------------------------------------------ autograd sees what is written
+def test_updates_in_place_are_seen_by_autograd(cuda):
+    """A graph that saved a tensor which one of the calls then writes refuses its backward pass, as after any update in place;
+    one whose tensors were read only goes through."""
+    def saved(t):
+        t = t.detach().requires_grad_(True)
+        u = t * 1.0                                       # not a leaf, so that it may be written
+        return u, (u * u).sum()
+
+    def changed(call, *shape):
+        u, loss = saved(rand(790, shape))
+        call(u)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+    w, x, target = rand(791, (32,)), rand(792, (6, 32)), torch.zeros(6, dtype=torch.int64, device="cuda")
+    rstd = ops.rms_norm(x, w)[2]
+    stats, d = ops.log_probs(x, target).stats, rand(793, (6,))
+    changed(lambda u: ops.rms_norm(x, w, out=u), 6, 32)
+    changed(lambda u: ops.rms_norm(x, w, residual=x, residual_out=u), 6, 32)
+    changed(lambda u: ops.rms_norm(u, w, out=u), 6, 32)
+    changed(lambda u: ops.rms_norm_backward(x, x, w, rstd, dx=u), 6, 32)
+    changed(lambda u: ops.rms_norm_backward(x, x, w, rstd, dweight=u), 32)
+    changed(lambda u: ops.log_probs_backward(x, target, stats, d, dx=u), 6, 32)
+    for bits in (32, 8):
+        changed(lambda u: ops.AdamW([u], state_bits=bits).step([x], rate=1e-2, t=1), 6, 32)
+    q = torch.empty(6, 32, device="cuda", dtype=torch.float8_e4m3fn)
+    before = q._version
+    ops.rms_norm_e4m3(x, w, out=q)
+    assert q._version > before
+    u, loss = saved(x)
+    for call in (lambda: ops.rms_norm(u, w, residual=u), lambda: ops.rms_norm_backward(u, u, w, rstd, dresidual=u),
+                 lambda: ops.log_probs(u, target), lambda: ops.log_probs_backward(u, target, stats, d),
+                 lambda: ops.AdamW([w.clone()]).step([u[0].detach()], rate=1e-2, t=1)):
+        call()
+    loss.backward()
+    with torch.inference_mode():                          # tensors without a counter
+        p = [torch.ones(8, device="cuda")]
+        ops.AdamW(p).step([p[0].clone()], rate=1e-2, t=1)
+        ops.rms_norm(p[0], out=p[0])
