@@ -1066,6 +1066,22 @@ def _grouped_rows(t: torch.Tensor, name: str):
     return 0, 0, _row_stride(t, name)
 
 
+def _aligned_rows(x: torch.Tensor, inner: int, outer: int, stride: int):
+    """A tensor of x's shape and type, its outer and its row stride: dense but for the few elements that put each row at the
+    same distance from a 16-byte boundary as x's (its rows as _grouped_rows has them)."""
+    shape, vec = x.shape, 16 // x.element_size()
+    n, first = shape[-1], x.data_ptr() % 16 // x.element_size()
+    stride = n + (stride - n) % vec
+    st, at = [1], stride                      # from the innermost dimension out
+    for k in range(len(shape) - 2, -1, -1):
+        if k == 0 and inner:
+            at += (outer - at) % vec
+            outer = at
+        st.insert(0, at)
+        at *= shape[k]
+    return torch.empty(first + max(at, n), device=x.device, dtype=x.dtype).as_strided(shape, st, first), outer, stride
+
+
 def _target(target: torch.Tensor, shape, dev: int):
     if not isinstance(target, torch.Tensor) or target.dtype not in (torch.int64, torch.int32) or not target.is_cuda:
         raise TypeError("target must be an int64 or int32 CUDA tensor")
@@ -1114,7 +1130,8 @@ def log_probs_backward(x: torch.Tensor, target: Optional[torch.Tensor], stats: t
                        dx: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of :func:`log_probs` with respect to ``x``, from the gradients of ``logp`` and of ``entropy`` (float32, one
     for each row; either may be missing).  ``stats`` and ``temperature`` are the forward call's.  ``dx`` may be ``x``;
-    without it the gradient gets x's own strides."""
+    without it the gradient is dense, but for the few elements that keep its rows at the distances of x's from a 16-byte
+    boundary."""
     shape, dtype, dev = x.shape, x.dtype, x.get_device()
     kind = _DTYPE.get(dtype)
     if kind is None or dev < 0 or dev != _current_device():
@@ -1128,15 +1145,19 @@ def log_probs_backward(x: torch.Tensor, target: Optional[torch.Tensor], stats: t
     if dlogp is not None and target is None:
         raise ValueError("dlogp without target")
     tp, is64 = _target(target, shape[:-1], dev) if target is not None else (None, 0)
-    given = dx is not None
+    given, xp = dx is not None, x.data_ptr()
     if not given:
-        dx = torch.empty_strided(shape, x.stride(), device=x.device, dtype=dtype)
-        inner, outer, stride = (0, 0, classes) if x.is_contiguous() else _grouped_rows(x, "x")
-        dx_outer, dx_stride = outer, stride
+        if xp % 16 == 0 and x.is_contiguous():
+            dx = torch.empty_strided(shape, x.stride(), device=x.device, dtype=dtype)
+            inner, outer, stride = 0, 0, classes
+            dx_outer, dx_stride = outer, stride
+        else:
+            inner, outer, stride = _grouped_rows(x, "x")
+            dx, dx_outer, dx_stride = _aligned_rows(x, inner, outer, stride)
     else:
         inner, outer, stride = _grouped_rows(x, "x")
         _, dx_outer, dx_stride = _grouped_rows(_like(dx, shape, dtype, dev, "dx"), "dx")
-    d = capi.LogProbsBackwardDesc(x.data_ptr(), tp, _dense_f32(stats, 3 * rows, dev, "stats"), _dense_f32(dlogp, rows, dev, "dlogp"),
+    d = capi.LogProbsBackwardDesc(xp, tp, _dense_f32(stats, 3 * rows, dev, "stats"), _dense_f32(dlogp, rows, dev, "dlogp"),
                                   _dense_f32(dentropy, rows, dev, "dentropy"), dx.data_ptr(), rows, inner, outer, stride, dx_outer,
                                   dx_stride, classes, kind, is64, temperature)
     rc = capi.lib().pxe_log_probs_backward(_raw_stream(dev), C.byref(d))

@@ -317,3 +317,35 @@ def test_updates_in_place_are_seen_by_autograd(cuda):
         p = [torch.ones(8, device="cuda")]
         ops.AdamW(p).step([p[0].clone()], rate=1e-2, t=1)
         ops.rms_norm(p[0], out=p[0])
+
+
+# ------------------------------------------------------------------------------------------------ gradients of slices
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_log_probs_gradient_of_a_slice_is_dense_and_aligned_like_it(cuda, dtype):
+    """The gradient of a few rows of a large tensor takes the memory of a few rows; its rows lie at x's distances from a
+    16-byte boundary, so that whole vectors are used; its values are those of the rows in a tensor of their own."""
+    big = rand(800, (6, 40, 1003), dtype, 2.0)
+    odd = rand(801, (6 * 1003 + 3,), dtype, 2.0)
+    wide = rand(802, (3, 4, 5, 1100), dtype, 2.0)
+    slices = [big[:, -1], big[:, 3:5], big[2], big[:, 7:8], big[1:2, :9], big[:, :, 5:900][:, 39], odd[3:].view(6, 1003), odd[1:1004],
+              wide[..., 7:1010], wide[:, :, 2:3, :64], wide[1, :, 4], big[:, :0], big.view(240, 1003)[::40, 1:]]
+    for x in slices:
+        lead, v = x.shape[:-1], x.shape[-1]
+        target = torch.randint(-1, v, lead, device="cuda", generator=gen(803))
+        r, (d, dh) = ops.log_probs(x, target), (rand(k, (lead.numel(),)).view(lead) for k in (804, 805))
+        dense = x.clone(memory_format=torch.contiguous_format)
+        want = ops.log_probs_backward(dense, target, r.stats, d, dentropy=dh)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        got = ops.log_probs_backward(x, target, r.stats, d, dentropy=dh)
+        used = torch.cuda.memory_allocated() - before
+        rows = x.numel() // v
+        assert used <= (rows * (v + 8) + len(x) * 8 + 8) * x.element_size() + 512
+        assert got.shape == x.shape
+        size = (d.abs() + dh.abs() * 20).double()[..., None]
+        within(got, want, 8 * U * size + half_step(dtype, want.double()) * 2)    # (the two may add up a row's elements alike or not)
+        if rows:
+            mine, theirs = got.view(got.shape) if got.dim() > 1 else got[None], x if x.dim() > 1 else x[None]
+            for index in torch.cartesian_prod(*[torch.arange(k) for k in theirs.shape[:-1]]).reshape(-1, theirs.dim() - 1)[:50]:
+                at = tuple(int(k) for k in index)
+                assert (mine[at].data_ptr() - theirs[at].data_ptr()) % 16 == 0
