@@ -963,7 +963,7 @@ int launch_backward(cudaStream_t s, ProbsBackParams& p)
     return vecs <= 512 ? launch_backward<T, 32>(s, p, vecs) : launch_backward<T, kBackThreads>(s, p, vecs);
 }
 
-// Rows of x or dx: the checked strides, and the span they cover as one row tensor.
+// Rows of x or dx: the checked strides; what the strides of a single row or a single group say is put aside.
 int check_rows(const char* name, const void* ptr, int size, long long rows, long long& inner, long long& outer, long long& stride, int classes)
 {
     PXE_REQUIRE(reinterpret_cast<uintptr_t>(ptr) % size == 0, "%s is not aligned to its elements", name);
@@ -971,6 +971,8 @@ int check_rows(const char* name, const void* ptr, int size, long long rows, long
     if (stride == 0) stride = classes;
     PXE_REQUIRE(inner > 0 && rows % inner == 0, "%s: %lld rows in groups of %lld", name, rows, inner);
     PXE_REQUIRE(stride >= classes, "%s: row stride %lld is less than %d classes", name, stride, classes);
+    if (rows == inner) outer = 0;
+    if (rows == 1) stride = classes;
     PXE_REQUIRE(rows == inner || outer >= (inner - 1) * stride + classes, "%s: outer stride %lld, a group covers %lld", name, outer, (inner - 1) * stride + classes);
     return PXE_OK;
 }

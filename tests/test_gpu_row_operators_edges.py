@@ -349,3 +349,18 @@ def test_log_probs_gradient_of_a_slice_is_dense_and_aligned_like_it(cuda, dtype)
             for index in torch.cartesian_prod(*[torch.arange(k) for k in theirs.shape[:-1]]).reshape(-1, theirs.dim() - 1)[:50]:
                 at = tuple(int(k) for k in index)
                 assert (mine[at].data_ptr() - theirs[at].data_ptr()) % 16 == 0
+
+
+def test_log_probs_gradient_in_place_whatever_unused_strides_say(cuda):
+    """The outer stride of a single group and the row stride of a single row say nothing: dx may be x, however they differ."""
+    import ctypes as C
+    from pixienn_b200 import capi
+    x, target = rand(810, (4, 100)), torch.tensor([1, 2, -1, 99], device="cuda")
+    r, d = ops.log_probs(x, target), rand(811, (4,))
+    want = ops.log_probs_backward(x, target, r.stats, d)
+    for rows, inner, outer, dx_outer, stride, dx_stride in ((4, 4, 400, 0, 100, 0), (4, 4, 7, 1 << 40, 100, 100), (1, 0, 0, 0, 100, 300), (1, 1, 5, 9, 200, 0)):
+        mine = x[:rows].clone()
+        desc = capi.LogProbsBackwardDesc(mine.data_ptr(), target.data_ptr(), r.stats.data_ptr(), d.data_ptr(), None, mine.data_ptr(), rows, inner,
+                                         outer, stride, dx_outer, dx_stride, 100, capi.F32, 1, 1.0)
+        capi.check(capi.lib().pxe_log_probs_backward(torch.cuda.current_stream().cuda_stream, C.byref(desc)))
+        assert torch.equal(mine, want[:rows])
