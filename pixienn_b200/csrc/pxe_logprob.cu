@@ -9,12 +9,13 @@
 // an instruction in 16 bits), rescales its sums only when the running maximum grows, and forms d = x * c - o with one
 // rounding from the origin o = fl(m * c), two elements an instruction (as S and U).  The origin's rounding is the same
 // shift for every element, up to half a unit of o, and is taken out of log2 S at the end: at |m c| <= 2^24 it is at most
-// 1/2.  Beyond, 2^shift would leave the range of a float (at m = -1e10 and temperature 1 the shift is 440), so that
-// partial sums under a maximum of m c < -2^24 take the origin 0 instead, from which all they hold adds 0 (a mask's finite
-// value, until the thread or another one meets more), and a row whose own maximum lies beyond +-2^24 / c is read again
-// with (x - m) * c, which neither overflows nor loses the row.  So is every row at temperatures above 72 or below 1e-7, and
-// one in fp16 under half the lowest value: values of -inf are held at -2^100 (the lowest value in fp16), so that a
-// probability of 0 adds 0 * d = 0 to U, and count for nothing only from further away.
+// 1/2.  Beyond, 2^shift would leave the range of a float (at m = -1e10 and temperature 1 the shift is 440).  A row whose own
+// maximum lies beyond +-2^24 / c is therefore read again with (x - m) * c, which neither overflows nor loses the row; and
+// partial sums under a maximum of m c < -2^25, which count for nothing in any other row (a mask's finite value, until the
+// thread or another one meets more), take the origin 0, from which all they hold adds 0.  Values of -inf are held at -2^100
+// (the lowest value in fp16), so that a probability of 0 adds 0 * d = 0 to U; what they count for is nothing only from
+// further away, so that a row in fp16 under half the lowest value, and every row at temperatures above 72 or below 1e-7, is
+// read again as well.
 //
 // The alternatives need no second pass over the row.  The k-th largest of the threads' own maxima is a lower bound of the
 // k-th largest value of all, and whatever reaches it lies with the threads whose maximum does: k of them, and those that
@@ -91,12 +92,12 @@ __device__ __forceinline__ float distance(float x, float m, float c) { return ma
 struct Part {
     float m, s, u;
 };
-constexpr float kFar = 16777216.0f;                        // of m * c: its rounding shifts the sums by half a unit, 2^(1/2) of them
+constexpr float kFar = 16777216.0f;                        // of a row's m * c; its rounding is up to a half, and 1 at twice that
 // (a product that is never contracted into what uses it: the origin's rounding has to be the same everywhere)
 __device__ __forceinline__ float origin_of(float m, float c)
 {
     const float o = __fmul_rn(m, c);
-    return o < -kFar ? 0.0f : o;
+    return o < -2.0f * kFar ? 0.0f : o;                    // (2^-kFar of a row that is not read again)
 }
 
 __device__ __forceinline__ void rescale(float& s, float& u, float from, float to)

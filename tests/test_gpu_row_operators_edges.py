@@ -94,6 +94,32 @@ def test_log_probs_of_many_rows_with_finite_masks(cuda, dtype, v):
             assert top == 0 or torch.equal(got.top_index[k:k + m], few.top_index[:m])
 
 
+@pytest.mark.parametrize("v", [1030, 2100, 9001, 70000])
+@pytest.mark.parametrize("temperature", [1.0, 0.125])
+def test_log_probs_around_the_limits_of_the_origin(cuda, v, temperature):
+    """Rows whose values lie on both sides of -2^24 and 2^24, and of twice that, in units of temperature / log2(e): none of their
+    terms may be lost, on whichever side a thread's, a block's or the row's maximum lies."""
+    edge = 2.0 ** 24 * temperature * math.log(2.0)
+    spread = rand(650, (1, v))[0] * 3 * temperature
+    rows = []
+    for at in (-edge, edge, -2 * edge, 2 * edge):
+        for off in (-12, -6, -3, 0, 3, 6, 12):
+            rows.append(at + off * temperature + spread)
+        rows.append((at + spread).sort().values)
+        rows.append((at + spread).sort(descending=True).values)
+    x = torch.stack(rows)
+    target = x.argmax(1)
+    target[1::3] = v // 2
+    for top in (0, 4):
+        r, lp = check_probs(x, target, temperature, top)
+    (_, h, _, _), _ = probs64(x, target, temperature, 0)
+    check_gradient(x, target, r, lp, h, temperature)
+    many = x.repeat(40, 1)
+    check_probs(many, target.repeat(40), temperature)
+    for k in (0, 3, 7, 8, 12):
+        check_probs(x[k:k + 1], target[k:k + 1], temperature, 4)
+
+
 # ------------------------------------------------------------------------------------------------ AdamW
 def test_adamw_refuses_a_state_that_was_replaced(cuda):
     """The step writes where the plan's state was when it was made: another tensor in one of its lists, another list, or other
