@@ -520,7 +520,8 @@ log_probs_kernel(const ProbsParams p)
         if (rank == 0) store_unused(p, row, t);
         return;
     }
-    Slice<T> s{RowView<T>(static_cast<const T*>(p.x) + row_offset<long long>(row, p.inner, p.outer_stride, p.row_stride), p.classes), 0, 0, rank == 0, rank == ranks - 1};
+    const long long offset = row_offset<long long>(row, p.inner, p.outer_stride, p.row_stride);
+    Slice<T> s{RowView<T>(static_cast<const T*>(p.x) + offset, p.classes), 0, 0, rank == 0, rank == ranks - 1};
     const RowView<T>& r = s.r;
     const int per = (r.nvec + ranks - 1) / ranks;
     s.v0 = min(rank * per, r.nvec);
@@ -974,7 +975,8 @@ int check_rows(const char* name, const void* ptr, int size, long long rows, long
     PXE_REQUIRE(stride >= classes, "%s: row stride %lld is less than %d classes", name, stride, classes);
     if (rows == inner) outer = 0;
     if (rows == 1) stride = classes;
-    PXE_REQUIRE(rows == inner || outer >= (inner - 1) * stride + classes, "%s: outer stride %lld, a group covers %lld", name, outer, (inner - 1) * stride + classes);
+    const long long covered = (inner - 1) * stride + classes;
+    PXE_REQUIRE(rows == inner || outer >= covered, "%s: outer stride %lld, a group covers %lld", name, outer, covered);
     return PXE_OK;
 }
 // What such a tensor covers, in two ways that each cover all of it: its groups, and (where a group is a whole number of rows
@@ -1031,7 +1033,8 @@ extern "C" int pxe_log_probs(pxe_stream_t stream, const pxe_log_probs_desc* dp)
         PXE_REQUIRE(reinterpret_cast<uintptr_t>(o.ptr) % 4 == 0, "log_probs: an output is not aligned to its elements");
         PXE_REQUIRE(o.ptr != d.x && o.ptr != d.target && !conflict(span, x) && !rows_conflict(span, target), "log_probs: an output overlaps an input");
         for (const auto& other : outs)
-            PXE_REQUIRE(&other == &o || !other.ptr || (other.ptr != o.ptr && !rows_conflict(span, {other.ptr, 1, 0, other.bytes})), "log_probs: two outputs overlap");
+            PXE_REQUIRE(&other == &o || !other.ptr || (other.ptr != o.ptr && !rows_conflict(span, {other.ptr, 1, 0, other.bytes})),
+                        "log_probs: two outputs overlap");
     }
     DeviceInfo di;
     { const int rc = device_info(&di); if (rc != PXE_OK) return rc; }
@@ -1064,8 +1067,9 @@ extern "C" int pxe_log_probs_backward(pxe_stream_t stream, const pxe_log_probs_b
     p.c = kLog2e / d.temperature; p.inv_temperature = 1.0f / d.temperature;
     const int size = dtype_bytes(d.type);
     long long inner = d.inner;
-    { const int rc = check_rows("log_probs_backward: x", d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes); if (rc != PXE_OK) return rc; }
-    { const int rc = check_rows("log_probs_backward: dx", d.dx, size, d.rows, inner, p.dx_outer_stride, p.dx_row_stride, d.classes); if (rc != PXE_OK) return rc; }
+    int rc = check_rows("log_probs_backward: x", d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes);
+    if (rc == PXE_OK) rc = check_rows("log_probs_backward: dx", d.dx, size, d.rows, inner, p.dx_outer_stride, p.dx_row_stride, d.classes);
+    if (rc != PXE_OK) return rc;
     const Cover x = cover(d.x, size, d.rows, p.inner, p.outer_stride, p.row_stride, d.classes);
     const Cover dx = cover(d.dx, size, d.rows, inner, p.dx_outer_stride, p.dx_row_stride, d.classes);
     PXE_REQUIRE(d.dx == d.x ? p.row_stride == p.dx_row_stride && p.outer_stride == p.dx_outer_stride : !conflict(dx, x),

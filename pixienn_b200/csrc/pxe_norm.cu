@@ -19,6 +19,7 @@ namespace pxe {
 namespace {
 
 constexpr int kMaxChannels = 262144;
+constexpr int kMaxGroup = 128;                             // channels that share a scale, but for whole rows
 // Rows of the weight gradient's workspace, one for each block: about 9.7 MB of them, but at least 148 and at most 1184 (one
 // and eight for each SM).
 inline int max_partials(int channels) { return std::max(148, std::min(1184, 2424832 / channels)); }
@@ -255,7 +256,7 @@ rms_norm_kernel(const NormParams p)
                     store(i, scale);
                 }
             }
-        } else {                                           // fp32 bits of |y| order as integers do, NaN above everything
+        } else if constexpr (32 * VEC < kMaxGroup) {       // fp32 bits of |y| order as integers do, NaN above everything
             unsigned int* gm = group_max + threadIdx.y * p.groups;
             for (int g = threadIdx.x; g < p.groups; g += blockDim.x) gm[g] = 0u;
             __syncthreads();
@@ -584,9 +585,9 @@ rms_norm_backward_long_kernel(const NormBackParams p)
 // whatever it moves).  Here one thread keeps `stages` rows of every input coming in with bulk copies.  A row's barrier in
 // its reduction says that all threads are done with the row before, whose place is then refilled.  Waits are bounded: where a
 // copy does not complete, the block leaves NaN in that row of dx, in all its later ones and in its part of dweight, starts
-// no further copy, and waits, bounded too, for those under way, which end in its shared memory.  16384 x 4096 bf16: 82 us, the copy rate, against 91 by the form
-// above; 4096 x 8192: 46 against 74; 16384 x 1024: 27.4 against 27.9.  (Several short rows to a stage, filled by a warp, were
-// slower than the form above: 44 against 28 us at 8192 x 2048.)
+// no further copy, and waits, bounded too, for those under way, which end in its shared memory.  16384 x 4096 bf16: 82 us,
+// the copy rate, against 91 by the form above; 4096 x 8192: 46 against 74; 16384 x 1024: 27.4 against 27.9.  (Several short
+// rows to a stage, filled by a warp, were slower than the form above: 44 against 28 us at 8192 x 2048.)
 constexpr int kMaxStages = 8;
 constexpr int kWaitLimit = 1 << 18;                        // tries of 4 us each: about a second
 
@@ -627,7 +628,10 @@ struct Ring {
         const uint32_t bar = shared_address(full + stage);
         for (int i = 0; i < kWaitLimit; ++i) {
             uint32_t done;
-            asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+            asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                         : "=r"(done)
+                         : "r"(bar), "r"(parity)
+                         : "memory");
             if (done) return true;
         }
         return false;
@@ -652,7 +656,8 @@ rms_norm_backward_ring_kernel(const NormBackParams p, int stages)
     if (threadIdx.x < 2) missing[threadIdx.x] = 0;
     ring.init();
     auto fill = [&](int stage, long long row) {
-        const void* const src[3] = {static_cast<const T*>(p.dy) + row * p.dys, static_cast<const T*>(p.h) + row * p.hs, static_cast<const T*>(p.dres) + row * p.rs};
+        const void* const src[3] = {static_cast<const T*>(p.dy) + row * p.dys, static_cast<const T*>(p.h) + row * p.hs,
+                                    static_cast<const T*>(p.dres) + row * p.rs};
         ring.fill<3>(stage, src, inputs, bytes);
     };
     const long long step = gridDim.x;
@@ -795,9 +800,10 @@ Layout layout_for(int vec, int size, int channels, bool few, bool backward)
     return l;
 }
 
-// The ring form takes rows of 2 to 16 KB in whole vectors (shorter ones would need more blocks than the workspace has rows), when there are enough of them to fill the card: a thread for each
-// vector, 1024 threads to an SM, and the stages that seven eighths of the shared memory hold.  (Rows of 32 KB leave room for
-// two stages: 121 us against 113 for the form above at 4096 x 16384 bf16.)
+// The ring form takes rows of 2 to 16 KB in whole vectors (shorter ones would need more blocks than the workspace has rows),
+// when there are enough of them to fill the card: a thread for each vector, 1024 threads to an SM, and the stages that seven
+// eighths of the shared memory hold.  (Rows of 32 KB leave room for two stages: 121 us against 113 for the form above at
+// 4096 x 16384 bf16.)
 struct RingLayout {
     int threads, blocks_per_sm, stages;
     size_t shared;
@@ -887,6 +893,13 @@ int launch_backward(cudaStream_t s, const NormBackParams& p, const Layout& l, un
     return PXE_OK;
 }
 
+template <typename T>
+int launch_backward_16(cudaStream_t s, const NormBackParams& p, const Layout& l, unsigned grid, int vec)
+{
+    if (vec == 8) return launch_backward<T, 8>(s, p, l, grid);
+    return vec == 2 ? launch_backward<T, 2>(s, p, l, grid) : launch_backward<T, 1>(s, p, l, grid);
+}
+
 // Elements per access: the whole 16 bytes, 4, or one element, whichever alignment, strides and channels allow.
 int vec_for(int access, int channels, int size)
 {
@@ -909,7 +922,7 @@ extern "C" int pxe_rms_norm(pxe_stream_t stream, const pxe_rms_norm_desc* dp)
     PXE_REQUIRE(d.rows >= 0 && d.channels > 0, "rms_norm: shape [%lld, %d]", d.rows, d.channels);
     PXE_REQUIRE((d.y != nullptr) != (d.q != nullptr), "rms_norm: exactly one of y and q is the destination");
     PXE_REQUIRE(d.eps >= 0.0f, "rms_norm: eps is negative or NaN");
-    PXE_REQUIRE(!d.q || d.group == 0 || d.group == 32 || d.group == 64 || d.group == 128, "rms_norm: group %d is not 0, 32, 64 or 128", d.group);
+    PXE_REQUIRE(!d.q || d.group == 0 || d.group == 32 || d.group == 64 || d.group == kMaxGroup, "rms_norm: group %d is not 0, 32, 64 or 128", d.group);
     if (d.channels > kMaxChannels) return set_error(PXE_ERR_UNSUPPORTED, "rms_norm: %d channels, at most %d", d.channels, kMaxChannels);
     if (d.rows == 0) return PXE_OK;
     PXE_REQUIRE(d.x != nullptr, "rms_norm: x is null");
@@ -1048,8 +1061,7 @@ extern "C" int pxe_rms_norm_backward(pxe_stream_t stream, const pxe_rms_norm_bac
         const long long blocks = (d.rows + l.rpb - 1) / l.rpb;
         grid = (unsigned)std::min<long long>(std::min<long long>(blocks, max_partials(C)), (long long)di.sm_count * std::max(1, 1024 / (l.tpr * l.rpb)));
         if (d.type == PXE_F32) rc = vec == 4 ? launch_backward<float, 4>(s, p, l, grid) : launch_backward<float, 1>(s, p, l, grid);
-        else if (d.type == PXE_BF16) rc = vec == 8 ? launch_backward<bf16, 8>(s, p, l, grid) : vec == 2 ? launch_backward<bf16, 2>(s, p, l, grid) : launch_backward<bf16, 1>(s, p, l, grid);
-        else rc = vec == 8 ? launch_backward<f16, 8>(s, p, l, grid) : vec == 2 ? launch_backward<f16, 2>(s, p, l, grid) : launch_backward<f16, 1>(s, p, l, grid);
+        else rc = d.type == PXE_BF16 ? launch_backward_16<bf16>(s, p, l, grid, vec) : launch_backward_16<f16>(s, p, l, grid, vec);
     }
     if (rc != PXE_OK || !d.dweight) return rc;
     cudaLaunchConfig_t cfg{};

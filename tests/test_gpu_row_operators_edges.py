@@ -125,7 +125,7 @@ def test_adamw_refuses_a_state_that_was_replaced(cuda):
     """The step writes where the plan's state was when it was made: another tensor in one of its lists, another list, or other
     memory behind a tensor is refused; copying into the state is what loads another one."""
     for bits in (32, 8):
-        params, grads = [rand(700, (300,), torch.bfloat16), rand(701, (70,), torch.bfloat16)], [rand(702, (300,), torch.bfloat16), rand(703, (70,), torch.bfloat16)]
+        params, grads = ([rand(seed + k, (n,), torch.bfloat16) for k, n in enumerate((300, 70))] for seed in (700, 702))
         plan = ops.AdamW(params, state_bits=bits, master=True)
         names = ["m", "v", "master"] + (["m_scale", "v_scale"] if bits == 8 else [])
         old = {name: list(getattr(plan, name)) for name in names}              # (kept, so that nothing is freed)
