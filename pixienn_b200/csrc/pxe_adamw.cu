@@ -248,9 +248,9 @@ __device__ __forceinline__ void one_unit(const Entry& e, long long first, int la
     u.work(e, first, lane, step, key);
 }
 
-// 64 M elements: fp32 with states in 32 bits 272 us, 1.07 of the copy rate; fp32 with states in 8 bits 158 us (1.06); bf16
-// with a master copy and states in 8 bits 158 us (1.06), without the copy 126 us (0.83, 12 bytes an element and as many
-// instructions).  With a seed 223, 208 and 204 us: bound by the instructions of the hash and the roundings.
+// 64 M elements in 16 tensors: fp32 with states in 32 bits 272 us, 1.07 of the copy rate; fp32 with states in 8 bits 164 us
+// (1.02); bf16 with a master copy and states in 8 bits 164 us (1.02), without the copy 130 us (0.80, 10 bytes an element and as
+// many instructions).  With a seed 236, 219 and 212 us: bound by the instructions of the hash and the roundings.
 // Blocks of an SM: four (64 registers a thread, nothing spilled), six for 16-bit parameters with states in 8 bits, whose
 // lanes have half the bytes under way (64 M bf16 parameters: 122 against 134 us, with a master copy 164 against 167; fp32
 // parameters with states in 8 bits 157 against 171 us at six).

@@ -119,7 +119,9 @@ __device__ __forceinline__ void unpack_e4m3(const typename RawOf<N>::type& raw, 
     }
 }
 
-// The scale of values up to `largest` and its reciprocal (the scale is a normal number, so that neither overflows).
+// The scale of values up to `largest` and its reciprocal (the scale is a normal number, so that neither overflows).  Products
+// in place of two divisions: a quotient is off by at most 5 units of 2^-24 of itself, so that a value as near as that to the
+// border between two codes may take the one or the other; its error is half a step either way.
 __device__ __forceinline__ float max_nan(float a, float b);
 __device__ __forceinline__ float e4m3_scale(float largest) { return max_nan(largest * (1.0f / kE4m3Max), kScaleMin); }
 __device__ __forceinline__ float e4m3_inverse(float scale) { return fast_rcp(scale); }
